@@ -19,9 +19,12 @@ PACK_BF16X3, PACK_F16 = 0, 1
 BIJ_IDENTITY, BIJ_SOFTPLUS, BIJ_EXP, BIJ_SOFTMAX_CENTERED, BIJ_FILL_SCALE_TRIL = 0, 1, 2, 3, 4
 PRIOR_NONE, PRIOR_NORMAL, PRIOR_HALFNORMAL, PRIOR_DIRICHLET, PRIOR_WISHART_TRIL = 0, 1, 2, 3, 4
 MAX_PARAM_BLOCKS = 16
+MAX_LOOKUPS = 8
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ID_TYPES = {torch.int32: 0, torch.int64: 1}
 NOALLOC_MAX_CHAINS = 256
 ERR_TOO_LARGE = -4
-ABI_VERSION = 112     # BVI_VERSION of include/bvi.h this binding was written against
+ABI_VERSION = 113     # BVI_VERSION of include/bvi.h this binding was written against
 
 
 class ParamBlock(ctypes.Structure):
@@ -121,6 +124,28 @@ def lib():
         l.bvi_linreg_recommended_format.argtypes = [i64, i32, i32, ctypes.POINTER(ctypes.c_int)]
         l.bvi_philox_uint32.argtypes = [u64, u64, i32, i32, i32, vp, vp]
         l.bvi_philox_normal.argtypes = [u64, u64, i32, i32, vp, vp]
+        szp, fp = ctypes.POINTER(sz), ctypes.POINTER(ctypes.c_int64)
+        vpp = ctypes.POINTER(vp)
+        l.bvi_lookup.argtypes = [vp, i32, i64, i64, i64, vp, i32, i64, f32, vp, vp]
+        l.bvi_lookup_plan_bytes.argtypes = [i64, i64, szp, szp]
+        l.bvi_lookup_plan.argtypes = [vp, i32, i64, i64, vp, sz, vp, sz, vp]
+        l.bvi_lookup_grad_ws_bytes.argtypes = [i64, i64, i64, szp]
+        l.bvi_lookup_grad.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, vp, vp, sz, vp]
+        l.bvi_grouped_packed_bytes.argtypes = [i64, i32, i32, fp, ctypes.c_uint, szp, szp]
+        l.bvi_grouped_pack.argtypes = [vp, vp, i64, i32, i32, fp, vpp, vpp, vp, sz, vp, sz, vp]
+        l.bvi_grouped_ws_bytes.argtypes = [i64, i32, i32, fp, i32, szp]
+        l.bvi_grouped_logp_grad.argtypes = [vp, i64, i32, i32, fp, ctypes.c_uint, vp, i32, vp, vp, vp, vp, sz, vp]
+        l.bvi_global_norm_ws_bytes.argtypes = [i32, szp]
+        l.bvi_global_norm.argtypes = [i32, vpp, fp, ctypes.POINTER(i32), vp, vp, sz, vp]
+        l.bvi_clip_by_global_norm.argtypes = [i32, vpp, vpp, fp, ctypes.POINTER(i32), f32, vp, vp, vp, sz, vp]
+        l.bvi_adam_step_ws_bytes.argtypes = [i32, fp, szp]
+        f64 = ctypes.c_double
+        l.bvi_adam_step.argtypes = [i32, vpp, vpp, vpp, vpp, fp, vp, f64, f64, f64, f64, f32, f32, vp, sz, vp]
+        for name in ('bvi_lookup', 'bvi_lookup_plan_bytes', 'bvi_lookup_plan', 'bvi_lookup_grad_ws_bytes',
+                     'bvi_lookup_grad', 'bvi_grouped_packed_bytes', 'bvi_grouped_pack', 'bvi_grouped_ws_bytes',
+                     'bvi_grouped_logp_grad', 'bvi_global_norm_ws_bytes', 'bvi_global_norm', 'bvi_clip_by_global_norm',
+                     'bvi_adam_step_ws_bytes', 'bvi_adam_step'):
+            getattr(l, name).restype = i32
         for name in ('bvi_constrain', 'bvi_posterior_assemble', 'bvi_leapfrog_pre', 'bvi_leapfrog_post',
                      'bvi_hmc_begin', 'bvi_hmc_end', 'bvi_hmc_fused', 'bvi_nuts_fused', 'bvi_rwm_fused', 'bvi_philox_uint32', 'bvi_philox_normal',
                      'bvi_leapfrog_mid', 'bvi_leapfrog_pre_chainwise', 'bvi_leapfrog_post_chainwise', 'bvi_nuts_begin',
@@ -374,3 +399,147 @@ def mvn_tril_logp_grad(Y, theta, parameterisation, ws: Workspace, want_grad=True
     check(lib().bvi_mvn_tril_logp_grad(_ptr(Y), n, d, int(parameterisation), _ptr(theta), c, _ptr(logp), _ptr(grad),
                                        _ref_ptr(logp_ref), _ptr(buf), buf.numel(), _stream()), 'bvi_mvn_tril_logp_grad')
     return logp, grad
+
+
+# ---- lookups, grouped regression, lists of tensors ----
+class _Here:
+    """Makes a tensor's device the current one for a call (most calls find it so)."""
+
+    def __init__(self, device):
+        self.other = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self.other is not None:
+            self.other.__exit__(*exc)
+
+
+def _scratch(nbytes, device):
+    """Scratch of one call, from torch's allocator: a later call on the stream may reuse it, a captured graph keeps its
+    own, and no two calls share it while they run."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def lookup(table, rows, width, row_stride, ids, scale, out):
+    with _Here(table.device) as st:
+        check(lib().bvi_lookup(table.data_ptr(), ELEMENT_TYPES[table.dtype], rows, width, row_stride, ids.data_ptr(),
+                               ID_TYPES[ids.dtype], ids.numel(), scale, out.data_ptr(), st), 'bvi_lookup')
+
+
+def lookup_plan(ids, rows):
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    check(lib().bvi_lookup_plan_bytes(rows, ids.numel(), ctypes.byref(a), ctypes.byref(b)), 'bvi_lookup_plan_bytes')
+    with _Here(ids.device) as st:
+        plan, ws = _scratch(a.value, ids.device), _scratch(b.value, ids.device)
+        check(lib().bvi_lookup_plan(ids.data_ptr(), ID_TYPES[ids.dtype], ids.numel(), rows, plan.data_ptr(), plan.numel(),
+                                    ws.data_ptr(), ws.numel(), st), 'bvi_lookup_plan')
+    return plan
+
+
+def lookup_grad(g, n, width, row_stride, plan, rows, scale, out):
+    a = ctypes.c_size_t(0)
+    check(lib().bvi_lookup_grad_ws_bytes(rows, width, n, ctypes.byref(a)), 'bvi_lookup_grad_ws_bytes')
+    with _Here(g.device) as st:
+        ws = _scratch(a.value, g.device)
+        check(lib().bvi_lookup_grad(g.data_ptr(), ELEMENT_TYPES[g.dtype], n, width, row_stride, plan.data_ptr(), rows,
+                                    scale, out.data_ptr(), ws.data_ptr(), ws.numel(), st), 'bvi_lookup_grad')
+
+
+def _pointers(ts):
+    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() if t is not None else None for t in ts])
+
+
+def _int64s(values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def grouped_pack(X, y, ids, rows, columns):
+    """bvi_grouped_pack: the rows in every lookup's order.  X[n, d] or None, ids a list of int32[n], columns a list of
+    float32[n] or None.  Returns (packed, mask of the columns that are there)."""
+    _check_f32_cuda(X, y, *columns)
+    n, d = y.shape[0], 0 if X is None else X.shape[1]
+    mask = sum(1 << l for l, z in enumerate(columns) if z is not None)
+    sizes = _int64s(rows)
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    check(lib().bvi_grouped_packed_bytes(n, d, len(rows), sizes, mask, ctypes.byref(a), ctypes.byref(b)),
+          'bvi_grouped_packed_bytes')
+    with _Here(y.device) as st:
+        packed, ws = _scratch(a.value, y.device), _scratch(b.value, y.device)
+        check(lib().bvi_grouped_pack(_ptr(X), _ptr(y), n, d, len(rows), sizes, _pointers(ids), _pointers(columns),
+                                     packed.data_ptr(), packed.numel(), ws.data_ptr(), ws.numel(), st), 'bvi_grouped_pack')
+    return packed, mask
+
+
+def grouped_ws_bytes(n, d, rows, n_chains):
+    a = ctypes.c_size_t(0)
+    check(lib().bvi_grouped_ws_bytes(n, d, len(rows), _int64s(rows), n_chains, ctypes.byref(a)), 'bvi_grouped_ws_bytes')
+    return int(a.value)
+
+
+def _tensor_list(tensors, what):
+    if not isinstance(tensors, (list, tuple)) or not tensors:
+        raise TypeError('%s takes a non-empty list of tensors' % what)
+    device = None
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.dtype not in ELEMENT_TYPES:
+            raise TypeError('%s takes float32, bfloat16 and float16 tensors, got %s'
+                            % (what, t.dtype if isinstance(t, torch.Tensor) else type(t).__name__))
+        if not t.is_cuda:
+            raise BviError('%s: tensors must be on the GPU (there is no CPU fallback); got %s' % (what, t.device))
+        if device is not None and t.device != device:
+            raise ValueError('%s: tensors on %s and on %s' % (what, device, t.device))
+        device = t.device
+    return device
+
+
+def _list_arguments(tensors):
+    n = len(tensors)
+    return (n, _pointers(tensors), _int64s([t.numel() for t in tensors]),
+            (ctypes.c_int * n)(*[ELEMENT_TYPES[t.dtype] for t in tensors]))
+
+
+def _norm_scratch(n, device):
+    a = ctypes.c_size_t(0)
+    check(lib().bvi_global_norm_ws_bytes(n, ctypes.byref(a)), 'bvi_global_norm_ws_bytes')
+    return _scratch(a.value, device)
+
+
+def global_norm(tensors):
+    """bvi_global_norm of contiguous tensors: a float32 scalar on their device."""
+    device = _tensor_list(tensors, 'global_norm')
+    with _Here(device) as st:
+        n, ptrs, sizes, types = _list_arguments(tensors)
+        norm, ws = torch.empty((), dtype=torch.float32, device=device), _norm_scratch(n, device)
+        check(lib().bvi_global_norm(n, ptrs, sizes, types, norm.data_ptr(), ws.data_ptr(), ws.numel(), st),
+              'bvi_global_norm')
+    return norm
+
+
+def clip_by_global_norm(tensors, outputs, clip_norm, use_norm=None):
+    """bvi_clip_by_global_norm of contiguous tensors into `outputs` (same shapes and types; may be the tensors
+    themselves); returns the norm."""
+    device = _tensor_list(tensors, 'clip_by_global_norm')
+    with _Here(device) as st:
+        n, ptrs, sizes, types = _list_arguments(tensors)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        ws = _norm_scratch(n, device) if use_norm is None else None
+        check(lib().bvi_clip_by_global_norm(n, ptrs, _pointers(outputs), sizes, types, clip_norm, _ptr(use_norm),
+                                            norm.data_ptr(), _ptr(ws), ws.numel() if ws is not None else 0, st),
+              'bvi_clip_by_global_norm')
+    return norm
+
+
+def adam_step(x, g, m, v, step_count, lr, b1, b2, eps, clip_norm, global_clip_norm):
+    """bvi_adam_step over lists of contiguous float32 tensors."""
+    device = x[0].device
+    with _Here(device) as st:
+        sizes, a = _int64s([t.numel() for t in x]), ctypes.c_size_t(0)
+        check(lib().bvi_adam_step_ws_bytes(len(x), sizes, ctypes.byref(a)), 'bvi_adam_step_ws_bytes')
+        ws = _scratch(a.value, device)
+        check(lib().bvi_adam_step(len(x), _pointers(x), _pointers(g), _pointers(m), _pointers(v), sizes,
+                                  step_count.data_ptr(), lr, b1, b2, eps, clip_norm, global_clip_norm, ws.data_ptr(),
+                                  ws.numel(), st), 'bvi_adam_step')

@@ -113,7 +113,7 @@ class Normal(Distribution):
 
     def sample(self, sample_shape=(), generator=None):
         shape = tuple(sample_shape) + tuple(self.batch_shape)
-        return self.loc + self.scale * torch.randn(shape, generator=generator)
+        return self.loc + self.scale * torch.randn(shape, generator=generator).to(self.loc.device)
 
 
 class HalfNormal(Distribution):

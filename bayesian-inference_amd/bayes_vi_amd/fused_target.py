@@ -199,6 +199,48 @@ class LinearRegression(FusedLogLikelihood):
                 _native._ptr(buf), buf.numel(), _native._stream())
 
 
+class GroupedRegression(FusedLogLikelihood):
+    """y_i ~ Normal(beta_0 + x_i . w + sum_l z_il u_l[ids_l[i]], scale); theta = (beta_0, w[D], scale, u_1[G_1], ...):
+    linear regression with group-level effects, the tables u_l looked up by `symbolic.gather`.  `ids`: one integer column
+    per lookup, `rows` the table sizes, `columns` (optional) what the looked-up entries are multiplied with.  The rows are
+    laid out once, in every lookup's sorted order."""
+
+    def __init__(self, X, y, ids, rows, columns=None, group=None):
+        super().__init__(y.device, group)
+        self.y = y.to(torch.float32).contiguous().reshape(-1)
+        self.n = self.y.shape[0]
+        self.rows = [int(r) for r in rows]
+        columns = [None] * len(self.rows) if columns is None else list(columns)
+        if not 1 <= len(self.rows) <= _native.MAX_LOOKUPS or len(ids) != len(self.rows) or len(columns) != len(self.rows):
+            raise ValueError('one id column (and one entry of `columns`) for each of 1 to %d tables' % _native.MAX_LOOKUPS)
+        X = None if X is None else X.to(torch.float32).reshape(self.n, -1).contiguous() if self.n else X.to(torch.float32)
+        self.d = 0 if X is None else X.shape[1]
+        if self.d > 64:
+            raise ValueError('at most 64 feature columns beside the group effects, got %d' % self.d)
+        self.n_params = self.d + 2 + sum(self.rows)
+        packed_ids = []
+        for i, r in zip(ids, self.rows):
+            if i.dtype not in _native.ID_TYPES or i.numel() != self.n or i.device != self.y.device:
+                raise ValueError('ids must be int32 or int64 [%d] on %s' % (self.n, self.y.device))
+            if r < 1 or (self.n and (int(i.min()) < 0 or int(i.max()) >= r)):
+                raise ValueError('group numbers must lie in [0, %d)' % r)
+            packed_ids.append(i.reshape(-1).to(torch.int32).contiguous())
+        z = []
+        for c in columns:
+            if c is not None and (c.numel() != self.n or c.device != self.y.device):
+                raise ValueError('columns must have %d entries on %s' % (self.n, self.y.device))
+            z.append(None if c is None else c.to(torch.float32).reshape(-1).contiguous())
+        self.packed, self.mask = _native.grouped_pack(X if self.d else None, self.y, packed_ids, self.rows, z)
+        self._sizes = _native._int64s(self.rows)
+
+    def _call(self, theta, logp, grad, relative=False):
+        c = theta.shape[0]
+        buf = self.ws.get(_native.grouped_ws_bytes(self.n, self.d, self.rows, c))
+        _launch(_native.lib().bvi_grouped_logp_grad, _native._ptr(self.packed), self.n, self.d, len(self.rows), self._sizes,
+                self.mask, _native._ptr(theta), c, _native._ptr(logp), _native._ptr(grad), self._ref(relative),
+                _native._ptr(buf), buf.numel(), _native._stream())
+
+
 class GaussianMixture1D(FusedLogLikelihood):
     """y_i ~ sum_k w_k Normal(loc_k, scale_k); theta = (weights[K], loc[K], scale[K]).
     exploratory_experiments/univariate-gaussian-mixture-test.ipynb cell 15."""

@@ -12,16 +12,24 @@ def kl_reverse(logu):
     return -logu
 
 
+# elements of a variable up to which bvi_clip_adam_step (one workgroup) is used
+ONE_WORKGROUP_MAX = 65536
+
+
 class _AdamState:
     """The update of tf.optimizers.Adam (the optimizer `VI.fit` defaults to, vi.py:77) on torch parameters:
         m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
         lr_t = lr sqrt(1 - b2^t) / (1 - b1^t);  x <- x - lr_t m / (sqrt(v) + epsilon)
-    (epsilon sits outside the bias correction, unlike torch.optim.Adam).  The step counter lives on the
-    parameters' device and nothing here reads it back, so a step can be recorded in a HIP graph."""
+    (epsilon sits outside the bias correction, unlike torch.optim.Adam), after all gradients together were clipped to
+    `global_clipnorm`, if given (tf.clip_by_global_norm).  The step counter lives on the parameters' device and nothing
+    here reads it back, so a step can be recorded in a HIP graph."""
 
-    def __init__(self, params, lr, betas, eps):
+    def __init__(self, params, lr, betas, eps, global_clipnorm=None):
         self.params = list(params)
         self.lr, (self.b1, self.b2), self.eps = lr, betas, eps
+        if global_clipnorm is not None and not float(global_clipnorm) > 0.0:
+            raise ValueError('global_clipnorm must be positive, got %r' % global_clipnorm)
+        self.global_clipnorm = None if global_clipnorm is None else float(global_clipnorm)
         dev = self.params[0].device if self.params else torch.device('cpu')
         self.t = torch.zeros((), dtype=torch.float64, device=dev)
         self.m = [torch.zeros_like(p) for p in self.params]
@@ -37,6 +45,13 @@ class _AdamState:
 
     @torch.no_grad()
     def step(self):
+        if self.global_clipnorm is not None:
+            grads = [p.grad for p in self.params if p.grad is not None]
+            if grads:
+                norm = torch.sqrt(sum((g.double() * g.double()).sum() for g in grads))
+                factor = torch.clamp(self.global_clipnorm / norm, max=1.0) + (norm - norm)    # NaN if norm is not finite
+                for g in grads:
+                    g.mul_(factor.to(g.dtype))
         self.t += 1
         lr_t = (self.lr * torch.sqrt(1.0 - self.b2 ** self.t) / (1.0 - self.b1 ** self.t)).to(torch.float32)
         for p, m, v in zip(self.params, self.m, self.v):
@@ -50,7 +65,8 @@ class _AdamState:
     def clip_and_step(self, clip_norm=1.0):
         """tf.clip_by_norm(grad, clip_norm) per variable (vi.py:70) followed by `step`.  On the GPU each variable is
         one launch of bvi_clip_adam_step (norm, clip, moments, update) instead of some seven element-wise kernels,
-        which is most of a step's launches for a flow with a few dozen small variables."""
+        which is most of a step's launches for a flow with a few dozen small variables.  With `global_clipnorm`, or a
+        variable too large for one workgroup, all variables go through bvi_adam_step together."""
         live = [(p, m, v) for p, m, v in zip(self.params, self.m, self.v) if p.grad is not None]
         on_device = bool(live) and all(p.is_cuda and p.dtype == torch.float32 and p.is_contiguous()
                                        and p.grad.is_contiguous() and p.grad.dtype == torch.float32 for p, _, _ in live)
@@ -59,6 +75,13 @@ class _AdamState:
                 for p, _, _ in live:     # without a host sync
                     p.grad.mul_(torch.clamp(clip_norm / (p.grad.norm() + 1e-30), max=1.0))
             self.step()
+            return
+        if self.global_clipnorm is not None or any(p.numel() > ONE_WORKGROUP_MAX for p, _, _ in live):
+            hyper = (self.lr, self.b1, self.b2, self.eps)
+            if self.global_clipnorm is None:      # the constants that bvi_clip_adam_step takes: same results to rounding
+                hyper = tuple(float(np.float32(h)) for h in hyper)
+            _native.adam_step([p.detach() for p, _, _ in live], [p.grad for p, _, _ in live], [m for _, m, _ in live],
+                              [v for _, _, v in live], self.t, *hyper, float(clip_norm), self.global_clipnorm or 0.0)
             return
         lib, ptr, st = _native.lib(), _native._ptr, _native._stream()
         with torch.no_grad():
@@ -70,13 +93,17 @@ class _AdamState:
 
 class Adam:
     """Optimizer description with the reference's spelling, tf.optimizers.Adam(learning_rate=...);
-    bound to the surrogate's parameters when `VI.fit` starts."""
+    bound to the surrogate's parameters when `VI.fit` starts.  `global_clipnorm`: the step first clips all gradients
+    together to this norm (they come clipped to norm 1 per variable from `VI.fit`, vi.py:70)."""
 
-    def __init__(self, learning_rate=0.001, beta_1=0.9, beta_2=0.999, epsilon=1e-7):
+    def __init__(self, learning_rate=0.001, beta_1=0.9, beta_2=0.999, epsilon=1e-7, global_clipnorm=None):
         self.learning_rate, self.betas, self.eps = learning_rate, (beta_1, beta_2), epsilon
+        if global_clipnorm is not None and not float(global_clipnorm) > 0.0:
+            raise ValueError('global_clipnorm must be positive, got %r' % global_clipnorm)
+        self.global_clipnorm = global_clipnorm
 
     def bind(self, params, capturable=False):
-        return _AdamState(params, self.learning_rate, self.betas, self.eps)
+        return _AdamState(params, self.learning_rate, self.betas, self.eps, self.global_clipnorm)
 
 
 class VI(Inference):
@@ -162,10 +189,7 @@ class VI(Inference):
             lp, gz = post.unconstrained_log_prob_and_grad(b['z'], True)
             _native.check(grads(s, pu, ptr(lp), ptr(gz), ptr(eps), ptr(scale), ptr(b['loss']), ptr(sur.loc.grad),
                                 ptr(scale.grad), st), 'bvi_advi_*_grads')
-            for i, (prm, m, v) in enumerate(zip(opt.params, opt.m, opt.v)):
-                _native.check(lib.bvi_clip_adam_step(prm.numel(), ptr(prm), ptr(prm.grad), ptr(m), ptr(v), ptr(opt.t),
-                                                     1 if i == 0 else 0, opt.lr, opt.b1, opt.b2, opt.eps, 1.0, st),
-                              'bvi_clip_adam_step')
+        opt.clip_and_step(1.0)
         return b['loss'].clone()
 
     def _step(self, opt, params, sample_size):

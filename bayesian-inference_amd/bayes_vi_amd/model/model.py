@@ -18,8 +18,9 @@ import torch
 from .. import bijectors as tfb
 from .. import distributions as tfd
 from .. import symbolic as sym
-from ..fused_target import (FusedLogLikelihood, GaussianMixture1D, GaussianMixtureFullCov, LinearRegression,
-                            MultivariateNormalTriL, NormalIID, Posterior, ShardedLogLikelihood)
+from ..fused_target import (FusedLogLikelihood, GaussianMixture1D, GaussianMixtureFullCov, GroupedRegression,
+                            LinearRegression, MultivariateNormalTriL, NormalIID, Posterior, ShardedLogLikelihood)
+from .._native import MAX_LOOKUPS as _MAX_LOOKUPS
 from ..utils import to_ordered_dict
 
 
@@ -164,10 +165,11 @@ class Model:
 
     def describe_likelihood(self, features=None):
         """Symbolic recognition only (no data touched, no GPU): returns a dict with
-        'family' in {'normal_iid', 'linreg', 'gmm1d', 'gmm_fullcov', 'mvn_tril'}, 'index' (kernel parameter j <- model flat
-        index, -1 = constant 0) and, for 'linreg', the design-column recipe:
+        'family' in {'normal_iid', 'linreg', 'grouped', 'gmm1d', 'gmm_fullcov', 'mvn_tril'}, 'index' (kernel parameter j <-
+        model flat index, -1 = constant 0) and, for 'linreg' and 'grouped', the design-column recipe:
         'columns' = [[(feature_key, coef), ...] per slope parameter] and 'offset' =
-        [(feature_key | None, coef), ...] terms to subtract from y."""
+        [(feature_key | None, coef), ...] terms to subtract from y; for 'grouped' also 'lookups' = [(feature_key of the
+        group numbers, table size, [(feature_key | None, coef), ...] the multiplier) per looked-up table]."""
         syms = {name: sym.ParamSym(name, n) for name, n in zip(self.param_names, self.block_sizes)}
         kwargs = dict(syms)
         if not self.is_generative_model:
@@ -194,10 +196,12 @@ class Model:
             if self.is_generative_model:
                 raise sym.UnsupportedLikelihood('a generative Normal likelihood must have loc = one scalar parameter')
             loc = sym.Affine.lift(dist.loc)
-            intercept, order, columns, offset = None, [], {}, []
+            intercept, order, columns, offset, lookups = None, [], {}, [], {}
             for p, f, c in loc.terms:
                 if p is None:
                     offset.append((f, c))
+                elif isinstance(p[1], sym.RowIndex):
+                    lookups.setdefault((p[0], p[1][0]), []).append((f, c))
                 elif f is None:
                     if c != 1.0 or intercept is not None:
                         raise sym.UnsupportedLikelihood('at most one intercept parameter with coefficient 1 is fused')
@@ -207,6 +211,15 @@ class Model:
                         columns[p] = []
                         order.append(p)
                     columns[p].append((f, c))
+            if lookups:
+                tables = [(name, key, terms, syms[name].size) for (name, key), terms in lookups.items()]
+                if len(tables) > _MAX_LOOKUPS:
+                    raise sym.UnsupportedLikelihood('at most %d gathered tables are fused' % _MAX_LOOKUPS)
+                index = [pidx(intercept) if intercept is not None else -1] + [pidx(p) for p in order] + [off[scale.name]]
+                for name, _, _, size in tables:
+                    index += range(off[name], off[name] + size)
+                return dict(family='grouped', index=index, columns=[columns[p] for p in order], offset=offset,
+                            lookups=[(key, size, terms) for _, key, terms, size in tables])
             if not order:
                 raise sym.UnsupportedLikelihood('regression likelihood uses no feature')
             index = [pidx(intercept) if intercept is not None else -1] + [pidx(p) for p in order] + [off[scale.name]]
@@ -249,18 +262,38 @@ class Model:
                                         % type(dist).__name__)
 
     def design_matrix(self, desc, features, targets):
-        """Materialises (X[N, D], y_adjusted[N]) of a 'linreg' description."""
-        if isinstance(features, dict):
-            col = lambda k: torch.as_tensor(features[k], dtype=torch.float32).reshape(-1)
-        else:
-            fmat = torch.as_tensor(features, dtype=torch.float32)
-            fmat = fmat[:, None] if fmat.dim() == 1 else fmat
-            col = lambda k: fmat[:, k]
+        """Materialises (X[N, D], y_adjusted[N]) of a 'linreg' or 'grouped' description."""
+        raw = self._feature_column(features)
+        col = lambda k: raw(k).to(torch.float32)
         y = torch.as_tensor(targets, dtype=torch.float32).reshape(-1).clone()
         for f, c in desc['offset']:
             y = y - (c if f is None else c * col(f).to(y.device))
+        if not desc['columns']:
+            return y.new_zeros(y.shape[0], 0), y
         X = torch.stack([sum(c * col(f) for f, c in terms) for terms in desc['columns']], -1)
         return X, y
+
+    @staticmethod
+    def _feature_column(features):
+        """Column by key, in the type it was given in (group numbers may be integers)."""
+        if isinstance(features, dict):
+            return lambda k: torch.as_tensor(features[k]).reshape(-1)
+        fmat = torch.as_tensor(features)
+        fmat = fmat[:, None] if fmat.dim() == 1 else fmat
+        return lambda k: fmat[:, k]
+
+    def lookup_columns(self, desc, features):
+        """(ids, multiplier or None) of every lookup of a 'grouped' description."""
+        raw = self._feature_column(features)
+        out = []
+        for key, _, terms in desc['lookups']:
+            ids = sym.whole_numbers(raw(key))
+            z = None
+            if any(f is not None or c != 1.0 for f, c in terms) or len(terms) > 1:
+                z = sum(c * (raw(f).to(torch.float32) if f is not None else torch.ones_like(ids, dtype=torch.float32))
+                        for f, c in terms)
+            out.append((ids, z))
+        return out
 
     @staticmethod
     def _to_device(t):
@@ -285,6 +318,12 @@ class Model:
         elif desc['family'] == 'mvn_tril':
             mode = _native.MVN_SCALE_TRIL if desc['parameterisation'] == 'scale_tril' else _native.MVN_CHOL_PRECISION_SOLVE
             inner = MultivariateNormalTriL(self._to_device(y.reshape(-1, desc['d'])), mode, group=group)
+        elif desc['family'] == 'grouped':
+            X, y_adj = self.design_matrix(desc, features, y)
+            cols = self.lookup_columns(desc, features)
+            inner = GroupedRegression(self._to_device(X), self._to_device(y_adj), [self._to_device(i) for i, _ in cols],
+                                      [size for _, size, _ in desc['lookups']],
+                                      [None if z is None else self._to_device(z) for _, z in cols], group=group)
         else:
             X, y_adj = self.design_matrix(desc, features, y)
             inner = LinearRegression(self._to_device(X), self._to_device(y_adj), group=group,

@@ -12,6 +12,7 @@ generic fallback path.
 
 Supported algebra on symbols: +, -, unary -, * by python numbers, parameter *
 feature products, `matvec(features, w)` / `features @ w` for a vector parameter,
+`gather(u, features['group'])` for a vector parameter indexed by a column of integers,
 and indexing `w[j]`, `features['name']`, `features[:, j]`.
 """
 from __future__ import annotations
@@ -162,6 +163,45 @@ def matvec(features, w):
         raise ValueError('matvec: %d feature columns but parameter %s has %d entries'
                          % (len(features.keys), w.name, w.size))
     return Affine([((w.name, j if w.size > 1 else None), features.keys[j], 1.0) for j in range(w.size)])
+
+
+class RowIndex(tuple):
+    """Index of a parameter that differs from row to row: the key of a feature column of integers."""
+
+
+def gather(params, indices):
+    """tf.gather(params, indices, axis=-1): the entry of a vector parameter that each row's group selects (a varying
+    intercept; times a feature, a varying slope).  Inside a likelihood `indices` is a feature column and the result an
+    expression for the regression's location; with concrete GPU tensors (posterior-predictive evaluation: params
+    [..., G], indices[N]) the values [..., N], through `embedding.lookup`."""
+    import torch
+    if isinstance(params, torch.Tensor) and isinstance(indices, torch.Tensor):
+        ids = whole_numbers(indices.reshape(-1))
+        if not params.is_cuda:                      # draws of a prior live on the host
+            if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= params.shape[-1]):
+                raise IndexError('gather: an index lies outside [0, %d)' % params.shape[-1])
+            return params[..., ids.to(params.device)]
+        from . import embedding
+        table = params.reshape(-1, params.shape[-1]).T
+        return embedding.lookup(table, ids.to(params.device)).T.reshape(tuple(params.shape[:-1]) + (ids.numel(),))
+    if not isinstance(params, ParamSym) or params.index is not None or not isinstance(indices, FeatureColumn):
+        raise UnsupportedLikelihood('gather(u, column) needs a whole vector parameter and one feature column')
+    return Affine([((params.name, RowIndex((indices.key,))), None, 1.0)])
+
+
+def whole_numbers(column):
+    """A feature column of group numbers as int64 (columns made from a data frame are float32)."""
+    import torch
+    if column.dtype in (torch.int32, torch.int64):
+        return column.long()
+    if column.is_floating_point():
+        ids = column.long()
+        if bool((ids.to(column.dtype) != column).any()):
+            raise ValueError('a column of group numbers holds values that are not whole')
+        if column.dtype == torch.float32 and ids.numel() and int(ids.abs().max()) > 1 << 24:
+            raise ValueError('group numbers beyond 2^24 are not exact in float32: give the column as integers')
+        return ids
+    raise TypeError('a column of group numbers must hold integers, got %s' % column.dtype)
 
 
 class CholeskySolveIdentity:

@@ -1,0 +1,506 @@
+// Gaussian linear regression with group-level effects, for all chains at once:
+//   eta_ci = b_c + sum_j w_cj x_ij + sum_l z_il u_l,c[group_l(i)],   y_i ~ Normal(eta_ci, s_c)
+//   logp_c      = -n log s - n/2 log(2 pi) - sum_i e_ci^2 / (2 s^2),   e = y - eta
+//   d b = sum_i e / s^2;  d w_j = sum_i e x_ij / s^2;  d s = -n / s + sum_i e^2 / s^3
+//   d u_l[v]    = sum over {i : group_l(i) = v} of z_il e / s^2        (the gradient of a table lookup by sorted ids)
+// theta_c = (b, w[d], s, u_1[rows_1], u_2[rows_2], ...).  z_l may be absent (ones: a varying intercept) or a column
+// (a varying slope).  A row whose group is outside [0, rows_l) has no effect of lookup l.
+//
+// The dataset is fixed, so its rows are laid out once per lookup in that lookup's sorted order (`packed`).  A pass over
+// the l-th copy walks the rows in that order, a wave per stretch of `span` rows, and ends a running sum wherever the
+// group changes: each group's sum is complete within a wave or split over neighbouring ones.  Walking along the rows,
+// every new stretch raises (group + wave), so that sum is a slot number of its own without any list, and group v's
+// slots are v + first wave .. v + last wave.  The lookups of the other tables are gathers in the same pass; nothing of
+// size rows x chains is ever written.  A second launch adds up the slots and the dense sums in a fixed order.
+#include "bvi_common.h"
+
+#include <math.h>
+
+namespace {
+
+constexpr int GR_WAVES = 4;             // waves per workgroup
+constexpr int GR_MAX_WAVES = 4096;      // stretches per pass: 16 waves per CU
+
+struct GrPass {                         // one lookup's copy of the rows
+  const float* y;
+  const float* X;                       // [n, D], columns beyond d are zero
+  const int32_t* id[BVI_MAX_LOOKUPS];   // group of every lookup in this order; id[own] ascends
+  const float* z[BVI_MAX_LOOKUPS];      // or NULL
+  const int32_t* start;                 // of the own lookup
+  int64_t rows[BVI_MAX_LOOKUPS];
+  int64_t offset[BVI_MAX_LOOKUPS];      // of u_l in theta
+  int64_t at[BVI_MAX_LOOKUPS];          // of u_l in the transposed tables
+  int own, lookups;
+};
+
+// CP chains x 64 / CP rows per wave.  FIRST: this pass also takes the sums that need every row once.
+template <int CP, int D, bool GRAD, bool FIRST>
+__global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPass a, int64_t n, int d, int64_t span, int C, int64_t P,
+                                                                const float* __restrict__ theta,
+                                                                const float* __restrict__ tables,
+                                                                float* __restrict__ slots, double* __restrict__ dense) {
+  constexpr int Q = 64 / CP;
+  constexpr int DD = D ? D : 1;
+  const int lane = threadIdx.x & 63, cl = lane % CP, q = lane / CP;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chain = blockIdx.y * CP + cl;
+  const bool live = chain < C;
+  const int c = live ? chain : C - 1;
+  const float* th = theta + (int64_t)c * P;
+  const float b = th[0];
+  float w[DD], gw[DD];
+#pragma unroll
+  for (int j = 0; j < DD; ++j) {
+    w[j] = j < d ? th[1 + j] : 0.f;
+    gw[j] = 0.f;
+  }
+  double sum_e = 0.0, sum_sq = 0.0;
+  const int own = a.own;
+  const int32_t* key = a.id[own];
+  const float* zown = a.z[own];
+  const int64_t wid = (int64_t)blockIdx.x * GR_WAVES + wave;
+  int64_t i0 = wid * span;
+  const int64_t end = i0 + span < n ? i0 + span : n;
+  while (i0 < end) {
+    const int64_t g = key[i0];
+    const bool inside = g >= 0 && g < a.rows[own];
+    int64_t e0 = inside ? (int64_t)a.start[g + 1] : end;
+    if (e0 > end) e0 = end;
+    const float u = !inside ? 0.f : tables ? tables[(a.at[own] + g) * C + c] : th[a.offset[own] + g];
+    float se = 0.f, sq = 0.f, su = 0.f;
+    for (int64_t i = i0 + q; i < e0; i += Q) {
+      float x[DD];
+      if (D > 0) {
+#pragma unroll
+        for (int j = 0; j < D; ++j) x[j] = a.X[i * D + j];
+      }
+      const float zo = zown ? zown[i] : 1.f;
+      float r = a.y[i] - b - u * zo;
+      for (int l = 0; l < a.lookups; ++l) {
+        if (l == own) continue;
+        const int64_t k = a.id[l][i];
+        if (k >= 0 && k < a.rows[l]) r -= tables[(a.at[l] + k) * C + c] * (a.z[l] ? a.z[l][i] : 1.f);
+      }
+      if (D > 0) {
+#pragma unroll
+        for (int j = 0; j < D; ++j) r = fmaf(-w[j], x[j], r);
+      }
+      if (FIRST) {
+        sq = fmaf(r, r, sq);
+        if (GRAD) {
+          se += r;
+          if (D > 0) {
+#pragma unroll
+            for (int j = 0; j < D; ++j) gw[j] = fmaf(r, x[j], gw[j]);
+          }
+        }
+      }
+      if (GRAD) su = fmaf(r, zo, su);
+    }
+    if (FIRST) {
+      sum_sq += (double)sq;
+      sum_e += (double)se;
+    }
+    if (GRAD && inside) {
+#pragma unroll
+      for (int off = CP; off < 64; off <<= 1) su += __shfl_xor(su, off, 64);
+      if (q == 0 && live) slots[(g + wid) * C + c] = su;
+    }
+    i0 = e0;
+  }
+  if (!FIRST) return;
+  // the workgroup's dense sums: [0] e^2, [1] e, [2 + j] e x_j
+  __shared__ double red[GR_WAVES][CP];
+  const int count = GRAD ? 2 + d : 1;
+  for (int k = 0; k < count; ++k) {
+    double v;
+    if (k == 0) v = sum_sq;
+    else if (k == 1) v = sum_e;
+    else {
+      float f = 0.f;
+#pragma unroll
+      for (int j = 0; j < DD; ++j) f = k - 2 == j ? gw[j] : f;
+      v = (double)f;
+    }
+#pragma unroll
+    for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+    __syncthreads();
+    if (q == 0) red[wave][cl] = v;
+    __syncthreads();
+    if (threadIdx.x < CP && blockIdx.y * CP + threadIdx.x < (unsigned)C) {
+      double t = 0.0;
+      for (int x = 0; x < GR_WAVES; ++x) t += red[x][threadIdx.x];
+      dense[((int64_t)blockIdx.x * count + k) * C + blockIdx.y * CP + threadIdx.x] = t;
+    }
+  }
+}
+
+// theta's tables [C, rows] -> [rows, C], 64 x 64 through LDS
+__global__ __launch_bounds__(256) void grouped_transpose_kernel(const float* __restrict__ theta, int64_t P, int64_t first,
+                                                                int64_t rows, int C, float* __restrict__ tables) {
+  __shared__ float tile[64][65];
+  const int64_t r0 = (int64_t)blockIdx.x * 64;
+  const int c0 = blockIdx.y * 64, lane = threadIdx.x & 63;
+  for (int k = threadIdx.x >> 6; k < 64; k += 4)
+    if (c0 + k < C && r0 + lane < rows) tile[k][lane] = theta[(int64_t)(c0 + k) * P + first + r0 + lane];
+  __syncthreads();
+  for (int k = threadIdx.x >> 6; k < 64; k += 4)
+    if (r0 + k < rows && c0 + lane < C) tables[(r0 + k) * C + c0 + lane] = tile[lane][k];
+}
+
+struct GrFinish {
+  const int32_t* start[BVI_MAX_LOOKUPS];
+  const float* slots[BVI_MAX_LOOKUPS];
+  int64_t rows[BVI_MAX_LOOKUPS];
+  int64_t offset[BVI_MAX_LOOKUPS];
+  int64_t tile_end[BVI_MAX_LOOKUPS];    // workgroups of the lookups up to this one, behind the dense ones
+  int lookups;
+};
+
+// Workgroup x < count: dense sum x.  Others: 1024 / CP groups of a table; a thread adds one group's slots for one
+// chain, the workgroup together those of a group with many.
+constexpr int GR_MANY = 64;
+template <int CP>
+__global__ __launch_bounds__(1024) void grouped_finish_kernel(GrFinish f, int64_t n, int d, int count, int64_t span,
+                                                              int n_blocks, int C, int64_t P,
+                                                              const float* __restrict__ theta,
+                                                              const double* __restrict__ dense,
+                                                              const double* __restrict__ logp_ref,
+                                                              float* __restrict__ logp, float* __restrict__ grad) {
+  constexpr int GT = 1024 / CP;
+  __shared__ double red[1024];
+  const int cl = threadIdx.x % CP, q = threadIdx.x / CP;
+  const int chain = blockIdx.y * CP + cl;
+  const int c = chain < C ? chain : C - 1;
+  const double s = (double)theta[(int64_t)c * P + 1 + d];
+  if ((int)blockIdx.x < count) {
+    const int k = blockIdx.x;
+    double v = 0.0;
+    for (int x = q; x < n_blocks; x += GT) v += dense[((int64_t)x * count + k) * C + c];
+    red[threadIdx.x] = v;
+    __syncthreads();
+    for (int h = GT / 2; h >= 1; h >>= 1) {
+      if (q < h) red[threadIdx.x] += red[threadIdx.x + h * CP];
+      __syncthreads();
+    }
+    if (q == 0 && chain < C) {
+      v = red[cl];
+      if (k == 0) {
+        const double level = logp_ref ? *logp_ref : 0.0;
+        logp[c] = (float)(-(double)n * log(s) - 0.5 * (double)n * BVI_LN2PI_D - 0.5 * v / (s * s) - level);
+        if (grad) grad[(int64_t)c * P + 1 + d] = (float)(v / (s * s * s) - (double)n / s);
+      } else {
+        grad[(int64_t)c * P + (k == 1 ? 0 : k - 1)] = (float)(v / (s * s));
+      }
+    }
+    return;
+  }
+  const int64_t tile = blockIdx.x - count;
+  int l = 0;
+  while (l + 1 < f.lookups && tile >= f.tile_end[l]) ++l;
+  const int64_t g0 = (tile - (l ? f.tile_end[l - 1] : 0)) * GT, g = g0 + q, rows = f.rows[l];
+  const float* slots = f.slots[l];
+  double v = 0.0;
+  int64_t first = 0, last = -1;
+  if (g < rows) {
+    const int64_t b = f.start[l][g], e = f.start[l][g + 1];
+    if (e > b) {
+      first = g + b / span;
+      last = g + (e - 1) / span;
+    }
+  }
+  const bool many = last - first >= GR_MANY;
+  if (!many)
+    for (int64_t k = first; k <= last; ++k) v += (double)slots[k * C + c];
+  // groups with many slots, one after the other by everyone (`many` of a group is the same in its CP threads)
+  __shared__ int queue[GT];
+  __shared__ int queued;
+  if (threadIdx.x == 0) queued = 0;
+  __syncthreads();
+  if (many && cl == 0) queue[atomicAdd(&queued, 1)] = q;        // the order only says which goes first
+  __syncthreads();
+  const int waiting = queued;
+  for (int x = 0; x < waiting; ++x) {
+    const int64_t gg = g0 + queue[x], b = f.start[l][gg], e = f.start[l][gg + 1];
+    double t = 0.0;
+    for (int64_t k = gg + b / span + q; k <= gg + (e - 1) / span; k += GT) t += (double)slots[k * C + c];
+    red[threadIdx.x] = t;
+    __syncthreads();
+    for (int h = GT / 2; h >= 1; h >>= 1) {
+      if (q < h) red[threadIdx.x] += red[threadIdx.x + h * CP];
+      __syncthreads();
+    }
+    if (q == queue[x]) v = red[cl];
+    __syncthreads();
+  }
+  // neighbouring threads write neighbouring groups of one chain
+  float* out = reinterpret_cast<float*>(red);
+  out[threadIdx.x] = (float)(v / (s * s));
+  __syncthreads();
+  const int wc = threadIdx.x / GT, wg = threadIdx.x % GT;
+  if (blockIdx.y * CP + wc < (unsigned)C && g0 + wg < rows)
+    grad[(int64_t)(blockIdx.y * CP + wc) * P + f.offset[l] + g0 + wg] = out[wg * CP + wc];
+}
+
+// ---- packing: copy l of the rows, in the order of its plan ----
+__global__ __launch_bounds__(256) void grouped_pack_kernel(const float* __restrict__ X, const float* __restrict__ y,
+                                                           int64_t n, int d, int D, const int32_t* __restrict__ order,
+                                                           float* __restrict__ Xo, float* __restrict__ yo) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t k = order[i];
+  yo[i] = y[k];
+  for (int j = 0; j < D; ++j) Xo[i * D + j] = j < d ? X[k * d + j] : 0.f;
+}
+__global__ __launch_bounds__(256) void grouped_pack_column_kernel(const int32_t* __restrict__ id,
+                                                                  const float* __restrict__ z, int64_t n,
+                                                                  const int32_t* __restrict__ order,
+                                                                  int32_t* __restrict__ ido, float* __restrict__ zo) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t k = order[i];
+  ido[i] = id[k];
+  if (zo) zo[i] = z[k];
+}
+__global__ __launch_bounds__(256) void grouped_pack_start_kernel(const int32_t* __restrict__ start, int64_t m,
+                                                                 int32_t* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < m) out[i] = start[i];
+}
+
+// ---- host ----
+int64_t words(int64_t n) { return (n + 63) / 64 * 64; }
+int padded_d(int d) { return d == 0 ? 0 : d <= 1 ? 1 : d <= 2 ? 2 : d <= 4 ? 4 : d <= 8 ? 8 : d <= 16 ? 16 : d <= 32 ? 32 : 64; }
+
+bool shape_ok(int64_t n, int d, int lookups, const int64_t* rows) {
+  if (n < 0 || d < 0 || lookups < 1 || !rows) return false;
+  for (int l = 0; l < lookups && l < BVI_MAX_LOOKUPS; ++l)
+    if (rows[l] < 1) return false;
+  return true;
+}
+bool shape_supported(int64_t n, int d, int lookups, const int64_t* rows) {
+  if (d > 64 || lookups > BVI_MAX_LOOKUPS || n > BVI_LOOKUP_MAX) return false;
+  for (int l = 0; l < lookups; ++l)
+    if (rows[l] > (1 << 25)) return false;               // threads of the finishing launch: 64 per row
+  return true;
+}
+
+// 4-byte words of one copy: start, y, X, and per lookup the groups and, where there is one, the column
+struct Layout {
+  int64_t start, y, X, id[BVI_MAX_LOOKUPS], z[BVI_MAX_LOOKUPS], all;
+};
+Layout layout(int64_t n, int d, int lookups, int64_t rows, unsigned columns) {
+  Layout t;
+  int64_t at = 0;
+  t.start = at; at += words(rows + 1);
+  t.y = at; at += words(n);
+  t.X = at; at += words(n * padded_d(d));
+  for (int l = 0; l < lookups; ++l) {
+    t.id[l] = at; at += words(n);
+    t.z[l] = -1;
+    if (columns >> l & 1u) { t.z[l] = at; at += words(n); }
+  }
+  t.all = at;
+  return t;
+}
+int64_t packed_words(int64_t n, int d, int lookups, const int64_t* rows, unsigned columns) {
+  int64_t all = 0;
+  for (int l = 0; l < lookups; ++l) all += layout(n, d, lookups, rows[l], columns).all;
+  return all;
+}
+
+int chain_lanes(int C) { return bvi_chain_pack(C); }
+// rows per wave: at least two per row lane, and as many as leave GR_MAX_WAVES waves busy
+int64_t span_of(int64_t n, int C) {
+  const int64_t least = 2 * (64 / chain_lanes(C)) > 16 ? 2 * (64 / chain_lanes(C)) : 16;
+  const int64_t even = (n + GR_MAX_WAVES - 1) / GR_MAX_WAVES;
+  return even > least ? even : least;
+}
+int64_t waves_of(int64_t n, int C) { const int64_t s = span_of(n, C); return n > 0 ? (n + s - 1) / s : 1; }
+int64_t blocks_of(int64_t n, int C) { return (waves_of(n, C) + GR_WAVES - 1) / GR_WAVES; }
+
+// 4-byte words of the workspace: the dense sums, the transposed tables, the slots of every lookup
+struct Space {
+  int64_t dense, tables, slots[BVI_MAX_LOOKUPS], all;
+};
+Space space(int64_t n, int d, int lookups, const int64_t* rows, int C) {
+  Space t;
+  int64_t at = 0;
+  t.dense = at; at += words(2 * blocks_of(n, C) * (2 + d) * C);
+  int64_t sum = 0;
+  for (int l = 0; l < lookups; ++l) sum += rows[l];
+  t.tables = at; at += lookups > 1 ? words(sum * C) : 0;
+  for (int l = 0; l < lookups; ++l) {
+    t.slots[l] = at;
+    at += words((rows[l] + GR_WAVES * blocks_of(n, C)) * C);
+  }
+  t.all = at;
+  return t;
+}
+
+template <int CP, int D, bool GRAD, bool FIRST>
+void launch_pass(const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P, const float* theta,
+                 const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
+  hipLaunchKernelGGL((grouped_kernel<CP, D, GRAD, FIRST>), dim3(blocks, bvi_ceil_div(C, CP)), dim3(64 * GR_WAVES), 0, s, a,
+                     n, d, span, C, P, theta, tables, slots, dense);
+}
+template <int CP, int D>
+void launch_pass_mode(bool grad, bool first, const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P,
+                      const float* theta, const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
+  if (!grad) launch_pass<CP, D, false, true>(a, n, d, span, C, P, theta, tables, slots, dense, blocks, s);
+  else if (first) launch_pass<CP, D, true, true>(a, n, d, span, C, P, theta, tables, slots, dense, blocks, s);
+  else launch_pass<CP, D, true, false>(a, n, d, span, C, P, theta, tables, slots, dense, blocks, s);
+}
+template <int CP>
+void launch_pass_d(int D, bool grad, bool first, const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P,
+                   const float* theta, const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
+#define GR_D(X) \
+  case X: launch_pass_mode<CP, X>(grad, first, a, n, d, span, C, P, theta, tables, slots, dense, blocks, s); break
+  switch (D) {
+    GR_D(0); GR_D(1); GR_D(2); GR_D(4); GR_D(8); GR_D(16); GR_D(32); GR_D(64);
+  }
+#undef GR_D
+}
+
+}  // namespace
+
+extern "C" {
+
+int bvi_grouped_packed_bytes(int64_t n, int d, int n_lookups, const int64_t* rows, unsigned columns, size_t* packed_bytes,
+                             size_t* ws_bytes) {
+  if (!packed_bytes || !ws_bytes || !shape_ok(n, d, n_lookups, rows)) return BVI_ERR_ARG;
+  if (!shape_supported(n, d, n_lookups, rows)) return BVI_ERR_UNSUPPORTED;
+  *packed_bytes = 4 * (size_t)packed_words(n, d, n_lookups, rows, columns);
+  size_t most = 0;
+  for (int l = 0; l < n_lookups; ++l) {
+    size_t plan, scratch;
+    bvi_lookup_plan_bytes(rows[l], n, &plan, &scratch);
+    most = plan + scratch > most ? plan + scratch : most;
+  }
+  *ws_bytes = most;
+  return BVI_OK;
+}
+
+int bvi_grouped_pack(const float* X, const float* y, int64_t n, int d, int n_lookups, const int64_t* rows,
+                     const int32_t* const* ids, const float* const* columns, void* packed, size_t packed_bytes, void* ws,
+                     size_t ws_bytes, void* stream) {
+  if (!shape_ok(n, d, n_lookups, rows) || (n > 0 && (!y || (d > 0 && !X) || !ids))) return BVI_ERR_ARG;
+  if (!shape_supported(n, d, n_lookups, rows)) return BVI_ERR_UNSUPPORTED;
+  unsigned mask = 0;
+  for (int l = 0; l < n_lookups; ++l) {
+    if (n > 0 && !ids[l]) return BVI_ERR_ARG;
+    if (columns && columns[l]) mask |= 1u << l;
+  }
+  size_t need, scratch;
+  bvi_grouped_packed_bytes(n, d, n_lookups, rows, mask, &need, &scratch);
+  if (!packed || packed_bytes < need || !ws || ws_bytes < scratch) return BVI_ERR_WORKSPACE;
+  const hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)((n + 255) / 256));
+  float* base = (float*)packed;
+  for (int l = 0; l < n_lookups; ++l) {
+    const Layout t = layout(n, d, n_lookups, rows[l], mask);
+    size_t plan_bytes, sort_bytes;
+    bvi_lookup_plan_bytes(rows[l], n, &plan_bytes, &sort_bytes);
+    const int st = bvi_lookup_plan(n > 0 ? ids[l] : nullptr, BVI_IDS_I32, n, rows[l], ws, plan_bytes,
+                                   (char*)ws + plan_bytes, sort_bytes, stream);
+    if (st) return st;
+    const int32_t* order = (const int32_t*)ws;
+    const int32_t* start = (const int32_t*)ws + 2 * words(n);
+    hipLaunchKernelGGL(grouped_pack_start_kernel, dim3((unsigned)((rows[l] + 256) / 256)), dim3(256), 0, s, start,
+                       rows[l] + 1, (int32_t*)(base + t.start));
+    if (n > 0) {
+      hipLaunchKernelGGL(grouped_pack_kernel, grid, dim3(256), 0, s, X, y, n, d, padded_d(d), order, base + t.X,
+                         base + t.y);
+      for (int k = 0; k < n_lookups; ++k)
+        hipLaunchKernelGGL(grouped_pack_column_kernel, grid, dim3(256), 0, s, ids[k],
+                           t.z[k] >= 0 ? columns[k] : nullptr, n, order, (int32_t*)(base + t.id[k]),
+                           t.z[k] >= 0 ? base + t.z[k] : nullptr);
+    }
+    base += t.all;
+  }
+  BVI_HIP_CHECK_LAUNCH();
+  return BVI_OK;
+}
+
+int bvi_grouped_ws_bytes(int64_t n, int d, int n_lookups, const int64_t* rows, int n_chains, size_t* ws_bytes) {
+  if (!ws_bytes || !shape_ok(n, d, n_lookups, rows) || n_chains < 1) return BVI_ERR_ARG;
+  if (!shape_supported(n, d, n_lookups, rows)) return BVI_ERR_UNSUPPORTED;
+  if (n_chains > BVI_GROUPED_MAX_CHAINS) return BVI_ERR_UNSUPPORTED;
+  *ws_bytes = 4 * (size_t)space(n, d, n_lookups, rows, n_chains).all;
+  return BVI_OK;
+}
+
+int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, const int64_t* rows, unsigned columns,
+                          const float* theta, int n_chains, float* logp, float* grad, const double* logp_ref, void* ws,
+                          size_t ws_bytes, void* stream) {
+  if (!packed || !shape_ok(n, d, n_lookups, rows) || !theta || n_chains < 1 || !logp) return BVI_ERR_ARG;
+  if (!shape_supported(n, d, n_lookups, rows)) return BVI_ERR_UNSUPPORTED;
+  if (n_chains > BVI_GROUPED_MAX_CHAINS) return BVI_ERR_UNSUPPORTED;
+  const int C = n_chains;
+  const Space t = space(n, d, n_lookups, rows, C);
+  if (!ws || ws_bytes < 4 * (size_t)t.all) return BVI_ERR_WORKSPACE;
+  const hipStream_t s = (hipStream_t)stream;
+  const int64_t span = span_of(n, C);
+  const int blocks = (int)blocks_of(n, C), cp = chain_lanes(C), count = grad ? 2 + d : 1;
+  int64_t P = d + 2, sum = 0;
+  for (int l = 0; l < n_lookups; ++l) P += rows[l];
+  float* w = (float*)ws;
+  double* dense = (double*)(w + t.dense);
+  const float* tables = nullptr;
+  if (n_lookups > 1) {
+    tables = w + t.tables;
+    hipLaunchKernelGGL(grouped_transpose_kernel, dim3((unsigned)((P - d - 2 + 63) / 64), bvi_ceil_div(C, 64)), dim3(256), 0,
+                       s, theta, P, (int64_t)(d + 2), P - d - 2, C, w + t.tables);
+  }
+  GrFinish f;
+  f.lookups = n_lookups;
+  const float* base = (const float*)packed;
+  int64_t tiles = 0;
+  for (int l = 0; l < n_lookups; ++l) {
+    const Layout p = layout(n, d, n_lookups, rows[l], columns);
+    if (l == 0 || grad) {
+      GrPass a;
+      a.y = base + p.y;
+      a.X = base + p.X;
+      a.start = (const int32_t*)(base + p.start);
+      a.own = l;
+      a.lookups = n_lookups;
+      int64_t at = 0;
+      for (int k = 0; k < n_lookups; ++k) {
+        a.id[k] = (const int32_t*)(base + p.id[k]);
+        a.z[k] = p.z[k] >= 0 ? base + p.z[k] : nullptr;
+        a.rows[k] = rows[k];
+        a.offset[k] = d + 2 + at;
+        a.at[k] = at;
+        at += rows[k];
+      }
+      float* slots = w + t.slots[l];
+#define GR_CP(X)                                                                                                      \
+  case X:                                                                                                             \
+    launch_pass_d<X>(padded_d(d), grad != nullptr, l == 0, a, n, d, span, C, P, theta, tables, slots, dense, blocks, s); \
+    break
+      switch (cp) { GR_CP(1); GR_CP(4); GR_CP(16); GR_CP(64); }
+#undef GR_CP
+    }
+    f.start[l] = (const int32_t*)(base + p.start);
+    f.slots[l] = w + t.slots[l];
+    f.rows[l] = rows[l];
+    f.offset[l] = d + 2 + sum;
+    sum += rows[l];
+    tiles += (rows[l] + 1024 / cp - 1) / (1024 / cp);
+    f.tile_end[l] = tiles;
+    base += p.all;
+  }
+  const dim3 grid((unsigned)(count + (grad ? tiles : 0)), bvi_ceil_div(C, cp));
+#define GR_CP(X)                                                                                                   \
+  case X:                                                                                                          \
+    hipLaunchKernelGGL(grouped_finish_kernel<X>, grid, dim3(1024), 0, s, f, n, d, count, span, blocks, C, P, theta, \
+                       (const double*)dense, logp_ref, logp, grad);                                                \
+    break
+  switch (cp) { GR_CP(1); GR_CP(4); GR_CP(16); GR_CP(64); }
+#undef GR_CP
+  BVI_HIP_CHECK_LAUNCH();
+  return BVI_OK;
+}
+
+}  // extern "C"

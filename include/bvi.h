@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define BVI_VERSION 112
+#define BVI_VERSION 113
 
 #define BVI_OK 0
 #define BVI_ERR_ARG (-1)          /* NULL pointer, negative size, bad enum        */
@@ -466,6 +466,71 @@ int bvi_rwm_fused(int family, const float* X, const float* y, int64_t n, int d, 
 int bvi_philox_uint32(uint64_t seed, uint64_t step, int stream_id, int n_chains, int n_blocks, uint32_t* out,
                       void* stream);
 int bvi_philox_normal(uint64_t seed, uint64_t step, int n_chains, int n_params, float* out, void* stream);
+
+/* ---- embedding lookup with scaling, and its gradient by sorted ids: tf.gather / tf.nn.embedding_lookup inside a
+ * likelihood or a surrogate's network.  table[rows, width] with any row stride >= width (elements), ids[n] int32 or
+ * int64; an id outside [0, rows) is padding: it reads zeros and takes no part in the gradient.
+ *   bvi_lookup            out[n, width] = scale * table[ids]; the product in float, rounded once
+ *   bvi_lookup_plan       what the gradient needs of the ids alone (a stable sort; int32 order[n], key[n],
+ *                         start[rows + 1]): once per dataset, or per call where the ids change
+ *   bvi_lookup_grad       grad_table[rows, width] = scale * the sums of grad_out's rows per id, in float, rounded once;
+ *                         every row is written (zeros where no id asks for it); no atomics, the same bits every time
+ * dtype is that of table, out, grad_out and grad_table.  rows, width and n at most BVI_LOOKUP_MAX. */
+#define BVI_TYPE_F32 0
+#define BVI_TYPE_BF16 1
+#define BVI_TYPE_F16 2
+#define BVI_IDS_I32 0
+#define BVI_IDS_I64 1
+#define BVI_LOOKUP_MAX 2147000000
+int bvi_lookup(const void* table, int dtype, int64_t rows, int64_t width, int64_t row_stride, const void* ids,
+               int ids_type, int64_t n, float scale, void* out, void* stream);
+int bvi_lookup_plan_bytes(int64_t rows, int64_t n, size_t* plan_bytes, size_t* ws_bytes);
+int bvi_lookup_plan(const void* ids, int ids_type, int64_t n, int64_t rows, void* plan, size_t plan_bytes, void* ws,
+                    size_t ws_bytes, void* stream);
+int bvi_lookup_grad_ws_bytes(int64_t rows, int64_t width, int64_t n, size_t* ws_bytes);
+int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, int64_t row_stride, const void* plan,
+                    int64_t rows, float scale, void* grad_table, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- Gaussian linear regression with group-level effects: the loss that reads such tables, with its gradient.
+ *   y_i ~ Normal(b + x_i . w + sum_l z_il u_l[ids_l[i]], s);  theta = (b, w[d], s, u_1[rows_1], u_2[rows_2], ...)
+ * z_l (columns[l]) may be NULL: ones.  An id outside [0, rows_l) has no effect.  d <= 64, n_lookups <=
+ * BVI_MAX_LOOKUPS, rows_l <= 2^25.  `rows`, `ids` and `columns` (arrays of n_lookups) are HOST arrays; `ids[l]` and
+ * `columns[l]` device pointers.  bvi_grouped_pack lays the rows out once per dataset, in every lookup's order;
+ * `columns` of the other calls has bit l set where columns[l] was given.  Conventions of logp, grad, logp_ref and shards
+ * as for the families above. */
+#define BVI_MAX_LOOKUPS 8
+#define BVI_GROUPED_MAX_CHAINS (1 << 20)
+int bvi_grouped_packed_bytes(int64_t n, int d, int n_lookups, const int64_t* rows, unsigned columns, size_t* packed_bytes,
+                             size_t* ws_bytes);
+int bvi_grouped_pack(const float* X, const float* y, int64_t n, int d, int n_lookups, const int64_t* rows,
+                     const int32_t* const* ids, const float* const* columns, void* packed, size_t packed_bytes, void* ws,
+                     size_t ws_bytes, void* stream);
+int bvi_grouped_ws_bytes(int64_t n, int d, int n_lookups, const int64_t* rows, int n_chains, size_t* ws_bytes);
+int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, const int64_t* rows, unsigned columns,
+                          const float* theta, int n_chains, float* logp, float* grad, const double* logp_ref, void* ws,
+                          size_t ws_bytes, void* stream);
+
+/* ---- operators over a list of tensors; the lists (pointers, sizes in elements, types) are HOST arrays, copied into
+ * the launches.  Sums of squares in double.
+ *   bvi_global_norm           *norm (device float) = sqrt of the sum over all tensors of their squares
+ *                             (tf.linalg.global_norm)
+ *   bvi_clip_by_global_norm   outputs[t] = tensors[t] * min(1, clip_norm / norm), rounded once; all NaN when the norm is
+ *                             not finite (tf.clip_by_global_norm).  outputs[t] may be tensors[t]; no two outputs may
+ *                             overlap.  use_norm (device float, or NULL): that norm instead of the list's own.  *norm
+ *                             (or NULL) receives the norm that was used.
+ *   bvi_adam_step             one step over all variables: each gradient clipped to clip_norm (<= 0: not), all of them
+ *                             jointly to global_clip_norm (<= 0: not), left clipped in grad, then the update of
+ *                             bvi_clip_adam_step; *step_count (device double) is t - 1 on entry and t afterwards. */
+int bvi_global_norm_ws_bytes(int n_tensors, size_t* ws_bytes);
+int bvi_global_norm(int n_tensors, const void* const* tensors, const int64_t* sizes, const int* dtypes, float* norm,
+                    void* ws, size_t ws_bytes, void* stream);
+int bvi_clip_by_global_norm(int n_tensors, const void* const* tensors, void* const* outputs, const int64_t* sizes,
+                            const int* dtypes, float clip_norm, const float* use_norm, float* norm, void* ws,
+                            size_t ws_bytes, void* stream);
+int bvi_adam_step_ws_bytes(int n_tensors, const int64_t* sizes, size_t* ws_bytes);
+int bvi_adam_step(int n_tensors, float* const* x, float* const* grad, float* const* m, float* const* v,
+                  const int64_t* sizes, double* step_count, double learning_rate, double beta_1, double beta_2,
+                  double epsilon, float clip_norm, float global_clip_norm, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

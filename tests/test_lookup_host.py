@@ -1,0 +1,168 @@
+"""Host side of the lookup / clipping / grouped-regression operators: what is refused before anything is launched, the
+C entry points' status codes, and how a likelihood with gathered group effects is recognised."""
+import collections
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import bayes_vi_amd.distributions as tfd
+from bayes_vi_amd import _native, embedding, linalg, symbolic as sym
+from bayes_vi_amd.inference.vi.vi import Adam
+from bayes_vi_amd.model import Model
+
+
+def test_python_refusals_without_a_gpu():
+    t, i = torch.zeros(4, 3), torch.zeros(5, dtype=torch.int64)
+    with pytest.raises(_native.BviError, match='no CPU fallback'):
+        embedding.lookup(t, i)
+    with pytest.raises(_native.BviError, match='no CPU fallback'):
+        embedding.LookupPlan(i, 4)
+    with pytest.raises(TypeError, match='int32 or int64'):
+        embedding.lookup(t, i.float())
+    with pytest.raises(TypeError, match='int32 or int64'):
+        embedding.lookup(t, [0, 1])
+    with pytest.raises(ValueError, match='rows, width'):
+        embedding.lookup(torch.zeros(2, 2, 2), i)
+    with pytest.raises(ValueError, match='no entries'):
+        embedding.lookup(torch.zeros(0, 3), i)
+    with pytest.raises(ValueError, match='shape'):
+        embedding.lookup_grad(torch.zeros(4, 3), i, 4)
+    with pytest.raises(ValueError, match='num_rows'):
+        embedding.lookup_grad(torch.zeros(5, 3), i, 0)
+    with pytest.raises(TypeError, match='list'):
+        linalg.global_norm(t)
+    with pytest.raises(ValueError, match='no tensor'):
+        linalg.clip_by_global_norm([None], 1.0)
+    with pytest.raises(_native.BviError, match='no CPU fallback'):
+        linalg.clip_by_global_norm([t], 1.0)
+    with pytest.raises(TypeError, match='float32'):
+        linalg.global_norm([t.double()])
+    for bad in (0.0, -1.0, float('nan')):
+        with pytest.raises(ValueError, match='positive'):
+            Adam(global_clipnorm=bad)
+
+
+def test_c_entry_points_refuse_before_launching():
+    """Every call here must return its status from the argument checks: the pointers are not device memory."""
+    lib = _native.lib()
+    p = ctypes.c_void_p(4096)
+    z = ctypes.c_size_t(0)
+    one = _native._int64s([3])
+    assert lib.bvi_lookup(None, 0, 4, 3, 3, p, 0, 5, 1.0, p, None) == -1
+    assert lib.bvi_lookup(p, 7, 4, 3, 3, p, 0, 5, 1.0, p, None) == -1
+    assert lib.bvi_lookup(p, 0, 4, 3, 2, p, 0, 5, 1.0, p, None) == -1          # row stride below the width
+    assert lib.bvi_lookup(p, 0, 4, 3, 3, p, 2, 5, 1.0, p, None) == -1
+    assert lib.bvi_lookup(p, 0, 4, 3, 3, p, 0, -1, 1.0, p, None) == -1
+    assert lib.bvi_lookup(p, 0, 4, 3, 3, None, 0, 0, 1.0, None, None) == 0     # no ids: nothing to do
+    assert lib.bvi_lookup_plan_bytes(0, 5, ctypes.byref(z), ctypes.byref(z)) == -1
+    assert lib.bvi_lookup_plan_bytes(1 << 31, 5, ctypes.byref(z), ctypes.byref(z)) == -2
+    assert lib.bvi_lookup_plan(p, 1, 5, 4, p, 16, p, 16, None) == -3
+    assert lib.bvi_lookup_plan(None, 1, 5, 4, p, 1 << 30, p, 1 << 30, None) == -1
+    assert lib.bvi_lookup_grad_ws_bytes(4, 0, 5, ctypes.byref(z)) == -1
+    assert lib.bvi_lookup_grad(p, 0, 5, 3, 3, None, 4, 1.0, p, p, 16, None) == -1
+    assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 4, 1.0, p, None, 0, None) == -3
+    ptrs, types = (ctypes.c_void_p * 1)(4096), (ctypes.c_int * 1)(0)
+    assert lib.bvi_global_norm(0, ptrs, one, types, p, p, 1 << 20, None) == -1
+    assert lib.bvi_global_norm(1, ptrs, one, (ctypes.c_int * 1)(9), p, p, 1 << 20, None) == -1
+    assert lib.bvi_global_norm(1, ptrs, one, types, p, p, 8, None) == -3
+    assert lib.bvi_global_norm(1, (ctypes.c_void_p * 1)(4097), one, types, p, p, 1 << 20, None) == -1    # misaligned
+    assert lib.bvi_clip_by_global_norm(1, ptrs, ptrs, one, types, 0.0, None, p, p, 1 << 20, None) == -1
+    assert lib.bvi_clip_by_global_norm(1, ptrs, ptrs, _native._int64s([-1]), types, 1.0, None, p, p, 1 << 20, None) == -1
+    assert lib.bvi_adam_step(1, ptrs, ptrs, ptrs, ptrs, one, p, .1, .9, .999, 1e-7, 1., 1., p, 8, None) == -3
+    assert lib.bvi_adam_step(1, ptrs, ptrs, ptrs, ptrs, one, None, .1, .9, .999, 1e-7, 1., 1., p, 1 << 20, None) == -1
+    assert lib.bvi_grouped_packed_bytes(5, 65, 1, one, 0, ctypes.byref(z), ctypes.byref(z)) == -2
+    assert lib.bvi_grouped_packed_bytes(5, 1, 9, _native._int64s([1] * 9), 0, ctypes.byref(z), ctypes.byref(z)) == -2
+    assert lib.bvi_grouped_packed_bytes(5, 1, 1, _native._int64s([0]), 0, ctypes.byref(z), ctypes.byref(z)) == -1
+    assert lib.bvi_grouped_ws_bytes(5, 1, 1, one, 0, ctypes.byref(z)) == -1
+    assert lib.bvi_grouped_ws_bytes(5, 1, 1, one, (1 << 20) + 1, ctypes.byref(z)) == -2
+    assert lib.bvi_grouped_logp_grad(p, 5, 1, 1, one, 0, p, 4, p, p, None, p, 16, None) == -3
+
+
+def _priors(**sizes):
+    return collections.OrderedDict((k, tfd.HalfNormal(1.) if k == 'scale' else tfd.Normal(0., 1.) if n == 0 else
+                                    tfd.Normal(torch.zeros(n), torch.ones(n))) for k, n in sizes.items())
+
+
+def test_recognise_varying_intercepts_and_slopes():
+    feats = dict(school=torch.zeros(6), x=torch.zeros(6), year=torch.zeros(6))
+    m = Model(_priors(mu=0, u=5, scale=0), lambda mu, u, scale, features: tfd.Normal(
+        loc=mu + sym.gather(u, features['school']), scale=scale))
+    d = m.describe_likelihood(feats)
+    assert d['family'] == 'grouped' and d['columns'] == []
+    assert d['index'] == [0, 6, 1, 2, 3, 4, 5]
+    assert d['lookups'] == [('school', 5, [(None, 1.0)])]
+    m = Model(_priors(mu=0, w=0, scale=0, u=3, v=4), lambda mu, w, scale, u, v, features: tfd.Normal(
+        loc=mu + w * features['x'] + 0.5 * sym.gather(u, features['school']) * features['x']
+        - sym.gather(v, features['year']) + 2.0 * features['x'], scale=scale))
+    d = m.describe_likelihood(feats)
+    assert d['index'] == list(range(10)) and d['columns'] == [[('x', 1.0)]] and d['offset'] == [('x', 2.0)]
+    assert d['lookups'] == [('school', 3, [('x', 0.5)]), ('year', 4, [(None, -1.0)])]
+    feats['x'] = torch.arange(6.)
+    feats['year'] = torch.tensor([0., 1., 2., 3., 0., 1.])
+    (i0, z0), (i1, z1) = m.lookup_columns(d, feats)
+    assert i1.dtype == torch.int64 and i1.tolist() == [0, 1, 2, 3, 0, 1]
+    assert torch.equal(z0, 0.5 * feats['x']) and torch.equal(z1, -torch.ones(6))
+    X, y = m.design_matrix(d, feats, torch.zeros(6))
+    assert torch.equal(X[:, 0], feats['x']) and torch.equal(y, -2.0 * feats['x'])
+    # two uses of one table with the same groups are one lookup
+    m = Model(_priors(mu=0, u=3, scale=0), lambda mu, u, scale, features: tfd.Normal(
+        loc=mu + sym.gather(u, features['school']) * features['x'] + sym.gather(u, features['school']), scale=scale))
+    assert m.describe_likelihood(feats)['lookups'] == [('school', 3, [('x', 1.0), (None, 1.0)])]
+
+
+def test_unsupported_uses_of_gather():
+    feats = dict(g=torch.zeros(6), x=torch.zeros(6))
+    bad = [lambda u, scale, features: tfd.Normal(loc=sym.gather(u[0], features['g']), scale=scale),
+           lambda u, scale, features: tfd.Normal(loc=sym.gather(u, u), scale=scale),
+           lambda u, scale, features: tfd.Normal(loc=sym.gather(u, features['g']) * u[0], scale=scale),
+           lambda u, scale, features: tfd.Normal(loc=0., scale=sym.gather(u, features['g']))]
+    for f in bad:
+        with pytest.raises(sym.UnsupportedLikelihood):
+            Model(_priors(u=3, scale=0), f).describe_likelihood(feats)
+    many = Model(_priors(u=3, scale=0), lambda u, scale, features: tfd.Normal(
+        loc=sum(sym.gather(u, features['g%d' % k]) for k in range(9)), scale=scale))
+    with pytest.raises(sym.UnsupportedLikelihood, match='at most 8'):
+        many.describe_likelihood({'g%d' % k: torch.zeros(6) for k in range(9)})
+
+
+def test_group_numbers():
+    assert sym.whole_numbers(torch.tensor([0., 3., 1.])).tolist() == [0, 3, 1]
+    with pytest.raises(ValueError, match='not whole'):
+        sym.whole_numbers(torch.tensor([0.5]))
+    with pytest.raises(ValueError, match='not whole'):
+        sym.whole_numbers(torch.tensor([float('nan')]))
+    with pytest.raises(ValueError, match='2\\^24'):
+        sym.whole_numbers(torch.tensor([2.0 ** 25]))
+    with pytest.raises(TypeError):
+        sym.whole_numbers(torch.tensor([True]))
+
+
+def test_gather_on_host_draws():
+    u = torch.arange(6.).reshape(2, 3)
+    assert torch.equal(sym.gather(u, torch.tensor([2., 0.])), u[:, [2, 0]])
+    with pytest.raises(IndexError):
+        sym.gather(u, torch.tensor([3.]))
+
+
+def test_global_clipnorm_on_the_host_path():
+    """`step` on CPU parameters: Keras' order, the joint clip before the moments."""
+    rng = np.random.default_rng(0)
+    p = [torch.nn.Parameter(torch.tensor(rng.normal(size=s), dtype=torch.float32)) for s in (3, (2, 2))]
+    g = [rng.normal(size=q.shape) for q in p]
+    opt = Adam(learning_rate=0.1, global_clipnorm=0.5).bind(p)
+    x0 = [q.detach().double().numpy().copy() for q in p]
+    for q, k in zip(p, g):
+        q.grad = torch.tensor(k, dtype=torch.float32)
+    opt.step()
+    f = min(1.0, 0.5 / np.sqrt(sum((k.astype(np.float32).astype(np.float64) ** 2).sum() for k in g)))
+    for q, k, x in zip(p, g, x0):
+        m, v = 0.1 * f * k, 0.001 * (f * k) ** 2
+        lr = 0.1 * np.sqrt(1 - 0.999) / (1 - 0.9)
+        # m, v, sqrt, quotient, product: 6 roundings of the step of size <= 0.1, one of the result
+        np.testing.assert_allclose(q.detach().double().numpy(), x - lr * m / (np.sqrt(v) + 1e-7), rtol=2e-7, atol=1e-6)
+    for q in p:
+        q.grad = torch.full_like(q, float('inf'))
+    opt.step()
+    assert all(torch.isnan(q).all() for q in p)
