@@ -129,8 +129,8 @@ def lib():
         l.bvi_lookup.argtypes = [vp, i32, i64, i64, i64, vp, i32, i64, f32, vp, vp]
         l.bvi_lookup_plan_bytes.argtypes = [i64, i64, szp, szp]
         l.bvi_lookup_plan.argtypes = [vp, i32, i64, i64, vp, sz, vp, sz, vp]
-        l.bvi_lookup_grad_ws_bytes.argtypes = [i64, i64, i64, szp]
-        l.bvi_lookup_grad.argtypes = [vp, i32, i64, i64, i64, vp, i64, f32, vp, vp, sz, vp]
+        l.bvi_lookup_grad_ws_bytes.argtypes = [i64, i64, i64, i32, szp]
+        l.bvi_lookup_grad.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, f32, vp, vp, sz, vp]
         l.bvi_grouped_packed_bytes.argtypes = [i64, i32, i32, fp, ctypes.c_uint, szp, szp]
         l.bvi_grouped_pack.argtypes = [vp, vp, i64, i32, i32, fp, vpp, vpp, vp, sz, vp, sz, vp]
         l.bvi_grouped_ws_bytes.argtypes = [i64, i32, i32, fp, i32, szp]
@@ -440,13 +440,15 @@ def lookup_plan(ids, rows):
     return plan
 
 
-def lookup_grad(g, n, width, row_stride, plan, rows, scale, out):
+def lookup_grad(g, n, width, row_stride, ids, plan, rows, scale, out):
+    """From `ids` (contiguous), or from a plan's buffer."""
     a = ctypes.c_size_t(0)
-    check(lib().bvi_lookup_grad_ws_bytes(rows, width, n, ctypes.byref(a)), 'bvi_lookup_grad_ws_bytes')
+    check(lib().bvi_lookup_grad_ws_bytes(rows, width, n, plan is not None, ctypes.byref(a)), 'bvi_lookup_grad_ws_bytes')
     with _Here(g.device) as st:
         ws = _scratch(a.value, g.device)
-        check(lib().bvi_lookup_grad(g.data_ptr(), ELEMENT_TYPES[g.dtype], n, width, row_stride, plan.data_ptr(), rows,
-                                    scale, out.data_ptr(), ws.data_ptr(), ws.numel(), st), 'bvi_lookup_grad')
+        check(lib().bvi_lookup_grad(g.data_ptr(), ELEMENT_TYPES[g.dtype], n, width, row_stride, ids.data_ptr(),
+                                    ID_TYPES[ids.dtype], plan.data_ptr() if plan is not None else None, rows, scale,
+                                    out.data_ptr(), ws.data_ptr(), ws.numel(), st), 'bvi_lookup_grad')
 
 
 def _pointers(ts):

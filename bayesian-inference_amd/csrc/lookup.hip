@@ -62,34 +62,47 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table
   }
 }
 
-// ---- the sort: least significant digit first, at most 8 bits per pass, stable ----------------------------------------
-constexpr int RS_THREADS = 256, RS_ITEMS = 16, RS_TILE = RS_THREADS * RS_ITEMS, RS_DIGITS = 256;
+// ---- the sort: least significant digit first, at most 11 bits per pass, stable ---------------------------------------
+// Few launches count more than bytes here: two passes cover four million rows.  A workgroup's tile is ROUNDS x 256
+// positions; up to SORT_FUSED workgroups the scatter launch adds up the counts of the others by itself, beyond that a
+// launch between the two does.
+constexpr int SORT_MAX_BITS = 11, SORT_MAX_DIGITS = 1 << SORT_MAX_BITS, SORT_FUSED = 128;
 
 // the sort key of position i: the id, or `rows` for padding; later passes read the keys of the pass before
 template <typename I>
-__device__ __forceinline__ uint32_t rs_key(const I* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t rows,
-                                           int64_t i) {
+__device__ __forceinline__ uint32_t sort_key(const I* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t rows,
+                                             int64_t i) {
   if (keys) return keys[i];
   const int64_t id = (int64_t)ids[i];
   return (uint32_t)(id >= 0 && id < rows ? id : rows);
 }
 
-template <typename I>
-__global__ __launch_bounds__(RS_THREADS) void sort_count_kernel(const I* __restrict__ ids,
-                                                                const uint32_t* __restrict__ keys, int64_t n,
-                                                                int64_t rows, int shift, uint32_t mask, int n_blocks,
-                                                                uint32_t* __restrict__ count) {
-  __shared__ uint32_t hist[RS_DIGITS];
-  hist[threadIdx.x] = 0;
+// count[d digit_stride + block block_stride] = the block's positions with digit d
+template <typename I, int ROUNDS>
+__global__ __launch_bounds__(256) void sort_count_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys,
+                                                         int64_t n, int64_t rows, int shift, int digits,
+                                                         int64_t digit_stride, int64_t block_stride,
+                                                         uint32_t* __restrict__ count) {
+  __shared__ uint32_t hist[SORT_MAX_DIGITS];
+  for (int d = threadIdx.x; d < digits; d += 256) hist[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * RS_TILE;
+  const int64_t base = (int64_t)blockIdx.x * (256 * ROUNDS) + threadIdx.x;
 #pragma unroll
-  for (int j = 0; j < RS_ITEMS; ++j) {
-    const int64_t i = base + j * RS_THREADS + threadIdx.x;
-    if (i < n) atomicAdd(&hist[(rs_key(ids, keys, rows, i) >> shift) & mask], 1u);   // integer counts: order-free
+  for (int j = 0; j < ROUNDS; ++j) {
+    const int64_t i = base + j * 256;
+    if (i < n) atomicAdd(&hist[(sort_key(ids, keys, rows, i) >> shift) & (digits - 1)], 1u);   // integers: order-free
   }
   __syncthreads();
-  count[(int64_t)threadIdx.x * n_blocks + blockIdx.x] = hist[threadIdx.x];
+  for (int d = threadIdx.x; d < digits; d += 256) count[d * digit_stride + blockIdx.x * block_stride] = hist[d];
+}
+
+__device__ __forceinline__ uint32_t inclusive_wave_sum(uint32_t v) {
+  const int lane = threadIdx.x & 63;
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t t = __shfl_up(v, off, 64);
+    if (lane >= off) v += t;
+  }
+  return v;
 }
 
 // workgroup d: exclusive sums of digit d's counts over the blocks, in place, and the digit's total
@@ -97,17 +110,13 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(int n_blocks, uint32_t* 
                                                         uint32_t* __restrict__ total) {
   __shared__ uint32_t wave_sum[4];
   uint32_t* c = count + (int64_t)blockIdx.x * n_blocks;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
   uint32_t carry = 0;
   for (int b0 = 0; b0 < n_blocks; b0 += 256) {
     const int b = b0 + threadIdx.x;
     const uint32_t own = b < n_blocks ? c[b] : 0u;
-    uint32_t v = own;
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t t = __shfl_up(v, off, 64);
-      if (lane >= off) v += t;
-    }
-    if (lane == 63) wave_sum[wave] = v;
+    const uint32_t v = inclusive_wave_sum(own);
+    if ((threadIdx.x & 63) == 63) wave_sum[wave] = v;
     __syncthreads();
     uint32_t before = carry, all = 0;
     for (int w = 0; w < 4; ++w) {
@@ -121,33 +130,75 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(int n_blocks, uint32_t* 
   if (threadIdx.x == 0) total[blockIdx.x] = carry;
 }
 
-// Each wave owns RS_TILE / 4 consecutive positions and ranks them 64 at a time: eight ballots give the lanes with the
-// same digit, a counter per wave and digit the earlier rounds'.  Positions are visited in ascending order: stable.
-template <typename I>
-__global__ __launch_bounds__(RS_THREADS) void sort_scatter_kernel(
-    const I* __restrict__ ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n,
-    int64_t rows, int shift, uint32_t mask, int n_blocks, const uint32_t* __restrict__ count,
-    const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out) {
-  __shared__ uint32_t seen[4][RS_DIGITS];
+// Each wave owns ROUNDS x 64 consecutive positions and ranks them 64 at a time: one ballot per bit gives the lanes with
+// the same digit, a counter per wave and digit the earlier rounds'.  Positions are visited in ascending order: stable.
+template <typename I, int ROUNDS, bool FUSED, int EACH>
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const I* __restrict__ ids, const uint32_t* __restrict__ keys,
+                                                           const uint32_t* __restrict__ vals, int64_t n, int64_t rows,
+                                                           int shift, int bits, int n_blocks,
+                                                           const uint32_t* __restrict__ count,
+                                                           const uint32_t* __restrict__ total,
+                                                           uint32_t* __restrict__ keys_out,
+                                                           uint32_t* __restrict__ vals_out) {
+  __shared__ uint32_t seen[4][SORT_MAX_DIGITS];
   __shared__ uint32_t wave_sum[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int w = 0; w < 4; ++w) seen[w][threadIdx.x] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * RS_TILE + wave * (RS_TILE / 4) + lane;
-  uint32_t key[RS_ITEMS], rank[RS_ITEMS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << bits;
+  for (int d = threadIdx.x; d < digits; d += 256)
 #pragma unroll
-  for (int j = 0; j < RS_ITEMS; ++j) {
+    for (int w = 0; w < 4; ++w) seen[w][d] = 0;
+  const int64_t base = (int64_t)blockIdx.x * (256 * ROUNDS) + wave * (64 * ROUNDS) + lane;
+  uint32_t key[ROUNDS], rank[ROUNDS];
+#pragma unroll
+  for (int j = 0; j < ROUNDS; ++j) {
     const int64_t i = base + j * 64;
-    key[j] = i < n ? rs_key(ids, keys, rows, i) : 0u;
+    key[j] = i < n ? sort_key(ids, keys, rows, i) : 0u;
   }
+  // where each wave's entries of digit d go: digits before d, d's entries of earlier blocks, of earlier waves.  Thread t
+  // takes EACH neighbouring digits.
+  uint32_t at[EACH], all[EACH] = {}, own = 0;
+  const int d0 = threadIdx.x * EACH;
+  if (d0 < digits) {
+    if (FUSED) {
+      uint32_t before[EACH] = {};
+      for (int b0 = 0; b0 < n_blocks; b0 += 16) {
+        Pack<uint32_t, EACH> c[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int b = b0 + u < n_blocks ? b0 + u : n_blocks - 1;
+          c[u] = *reinterpret_cast<const Pack<uint32_t, EACH>*>(count + (int64_t)b * digits + d0);
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+#pragma unroll
+          for (int k = 0; k < EACH; ++k) {
+            all[k] += b0 + u < n_blocks ? c[u].e[k] : 0u;
+            before[k] += b0 + u < (int)blockIdx.x ? c[u].e[k] : 0u;
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) at[k] = before[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        all[k] = total[d0 + k];
+        at[k] = count[(int64_t)(d0 + k) * n_blocks + blockIdx.x];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      at[k] += own;
+      own += all[k];
+    }
+  }
+  __syncthreads();
   volatile uint32_t* mine = seen[wave];
 #pragma unroll
-  for (int j = 0; j < RS_ITEMS; ++j) {
+  for (int j = 0; j < ROUNDS; ++j) {
     const bool in = base + j * 64 < n;
-    const uint32_t d = (key[j] >> shift) & mask;
+    const uint32_t d = (key[j] >> shift) & (digits - 1);
     uint64_t same = __ballot(in);
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < SORT_MAX_BITS; ++b) {
       const uint64_t bit = __ballot((d >> b) & 1u);
       same &= ((d >> b) & 1u) ? bit : ~bit;
     }
@@ -159,170 +210,341 @@ __global__ __launch_bounds__(RS_THREADS) void sort_scatter_kernel(
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  // where each wave's entries of digit d go: digits before d, d's entries of earlier blocks, of earlier waves
-  const int d = threadIdx.x;
-  const uint32_t own = total[d];
-  uint32_t v = own;
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint32_t t = __shfl_up(v, off, 64);
-    if (lane >= off) v += t;
-  }
+  const uint32_t v = inclusive_wave_sum(own);
   if (lane == 63) wave_sum[wave] = v;
   __syncthreads();
-  uint32_t at = v - own + count[(int64_t)d * n_blocks + blockIdx.x];
-  for (int w = 0; w < wave; ++w) at += wave_sum[w];
-  for (int w = 0; w < 4; ++w) {
-    const uint32_t c = seen[w][d];
-    seen[w][d] = at;
-    at += c;
+  uint32_t first = v - own;
+  for (int w = 0; w < wave; ++w) first += wave_sum[w];
+  if (d0 < digits) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      uint32_t to = first + at[k];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t c = seen[w][d0 + k];
+        seen[w][d0 + k] = to;
+        to += c;
+      }
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < RS_ITEMS; ++j) {
+  for (int j = 0; j < ROUNDS; ++j) {
     const int64_t i = base + j * 64;
     if (i < n) {
-      const uint32_t to = seen[wave][(key[j] >> shift) & mask] + rank[j];
+      const uint32_t to = seen[wave][(key[j] >> shift) & (digits - 1)] + rank[j];
       keys_out[to] = key[j];
       vals_out[to] = vals ? vals[i] : (uint32_t)i;
     }
   }
 }
 
-// start[r] = number of sorted keys below r
-__global__ __launch_bounds__(256) void sort_start_kernel(const uint32_t* __restrict__ key, int64_t n, int64_t rows,
+// ---- few positions: each one's place is the number of positions sorted before it, counted against all of them --------
+// n^2 comparisons, two instructions each, over the whole chip and in one launch.  Eight neighbouring lanes share a
+// position and take every eighth vector of four keys.
+constexpr int RANK_MAX = 4096;
+template <typename I>
+__global__ __launch_bounds__(256) void sort_rank_kernel(const I* __restrict__ ids, int n, int64_t rows,
+                                                        uint32_t* __restrict__ order, uint32_t* __restrict__ key_out) {
+  __shared__ uint4 keys4[RANK_MAX / 4];
+  uint32_t* keys = reinterpret_cast<uint32_t*>(keys4);
+  const int vectors = (n + 31) / 32 * 8;
+  for (int j0 = threadIdx.x; j0 < vectors * 4; j0 += 256 * 8) {       // eight loads in flight
+    uint32_t k[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = j0 + u * 256;
+      k[u] = sort_key(ids, (const uint32_t*)nullptr, rows, j < n ? j : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = j0 + u * 256;
+      if (j < vectors * 4) keys[j] = j < n ? k[u] : 0xffffffffu;
+    }
+  }
+  __syncthreads();
+  const int i = blockIdx.x * 32 + (threadIdx.x >> 3), part = threadIdx.x & 7;
+  const uint32_t k = i < n ? keys[i] : 0u;
+  uint32_t place = 0;
+#pragma unroll 4
+  for (int v = part; v < vectors; v += 8) {
+    const uint4 x = keys4[v];
+    const uint32_t below = v < (i >> 2) ? k + 1u : k;          // equal keys in front of i count too
+    place += (x.x < below ? 1u : 0u) + (x.y < below ? 1u : 0u) + (x.z < below ? 1u : 0u) + (x.w < below ? 1u : 0u);
+  }
+  if (part == 0 && i < n)
+    for (int j = i & ~3; j < i; ++j) place += keys[j] == k ? 1u : 0u;     // and those in i's own vector
+  place += __shfl_xor(place, 1, 64);
+  place += __shfl_xor(place, 2, 64);
+  place += __shfl_xor(place, 4, 64);
+  if (part == 0 && i < n) {
+    order[place] = (uint32_t)i;
+    key_out[place] = k;
+  }
+}
+
+// start[r] = number of sorted keys below r.  With at least as many positions as rows: position p fills in the rows between
+// its neighbour's and its own, a wave together where those are many.
+__global__ __launch_bounds__(256) void sort_fill_start_kernel(const uint32_t* __restrict__ key, int64_t n, uint32_t rows,
+                                                              int32_t* __restrict__ start) {
+  const int64_t p = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const uint32_t from = p == 0 || p > n ? 0u : key[p - 1] + 1u;      // rows [from, to] start at p
+  const uint32_t to = p < n ? key[p] : rows;
+  const uint32_t gap = p <= n && to + 1u > from ? to + 1u - from : 0u;
+  if (gap <= 8)
+    for (uint32_t r = 0; r < gap; ++r) start[from + r] = (int32_t)p;
+  for (uint64_t wide = __ballot(gap > 8); wide; wide &= wide - 1ull) {
+    const int src = __ffsll((unsigned long long)wide) - 1;
+    const uint32_t f = __shfl(from, src, 64), m = __shfl(gap, src, 64);
+    const int32_t at = (int32_t)(p - lane + src);
+    for (uint32_t r = lane; r < m; r += 64) start[f + r] = at;
+  }
+}
+
+// With fewer: a search per row.  Sixteen probes at a time: the search waits for loads, not for their number.
+__global__ __launch_bounds__(256) void sort_start_kernel(const uint32_t* __restrict__ key, int n, int64_t rows,
                                                          int32_t* __restrict__ start) {
   const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (r > rows) return;
-  int64_t lo = 0, hi = n;
+  int lo = 0, hi = n;                              // the answer lies in [lo, hi]
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if ((int64_t)key[mid] < r) lo = mid + 1;
-    else hi = mid;
+    const int step = (hi - lo + 15) >> 4;
+    uint32_t k[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int at = lo + (u + 1) * step - 1;      // below 2^31: n has room for a step more
+      k[u] = key[at < hi ? at : hi - 1];
+    }
+    int below = 0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) below += lo + (u + 1) * step - 1 < hi && (int64_t)k[u] < r ? 1 : 0;
+    lo += below * step;
+    hi = below == 16 ? lo : min(hi, lo + step - 1);
   }
-  start[r] = (int32_t)lo;
+  start[r] = lo;
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------
-// A wave is LE lanes across the columns times 64 / LE lanes over positions.  A row read at most a few hundred times is
-// one wave's work; where a row has more, whole blocks of `chunk` sorted positions that belong to it ("pure" blocks) are
-// summed beforehand by a wave each, and blocks of 64 pure blocks once more.
-constexpr int LG_FAN = 64;
+// So that no thread has many positions of one row to add: blocks of 2^chunk_bits sorted positions that belong to one row
+// are summed beforehand (level 1), blocks of 2^fan_bits of those again (level 2), and so on; a row adds the entries at
+// its ends one by one and whole blocks in between.  Two forms of the three kernels:
+//   wide rows, or few positions per row: a thread per vector of V columns, two or three positions in flight (more cost
+//   the registers of a wave that hides as much: 65537 x 640 bf16 into 100003 rows 66 us with four, 41 with two, which is
+//   5.2 TB/s);
+//   narrow rows: a wave per row, LE lanes across the columns times Q = 64 / LE over the positions (2M x 16 into 5000 rows
+//   14 us after 29 us for the blocks of 128; a thread per vector took 43 after 42).
+constexpr int GRAD_LEVELS = 8;
+struct GradLevels {
+  int count, chunk_bits, fan_bits;
+  int64_t n[GRAD_LEVELS];             // blocks of the level
+  int64_t at[GRAD_LEVELS];            // where its sums start in the workspace (floats)
+};
 
-// acc += rows src[order[p]] for p in [s, e); lane q takes p = s + q, s + q + Q, ...; four loads in flight
-template <typename S, int V, int LE, bool PERM>
-__device__ __forceinline__ void lg_sum(float (&acc)[V], const S* __restrict__ src, int64_t stride, int64_t col,
-                                       const int32_t* __restrict__ order, int64_t s, int64_t e, int q, bool active) {
-  constexpr int Q = 64 / LE;
-  if (!active) return;
-  int64_t p = s + q;
-  for (; p + 3 * Q < e; p += 4 * Q) {
-    Pack<S, V> x[4];
+__host__ __device__ __forceinline__ int64_t level_space(int64_t floats) { return (floats + 63) / 64 * 64; }
+
+// acc += columns [col, col + V) of the rows src[order[p]] (or src[p] without an order), p = a, a + Q, ... below b
+template <typename S, int V, bool PERM, int Q, int DEEP>
+__device__ __forceinline__ void grad_sum(float (&acc)[V], const S* __restrict__ src, int64_t stride, int64_t col,
+                                         const int32_t* __restrict__ order, int a, int b) {
+  for (int p = a; p < b; p += DEEP * Q) {
+    Pack<S, V> x[DEEP];
+    int32_t i[DEEP];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = PERM ? (int64_t)order[p + u * Q] : p + u * Q;
-      x[u] = *reinterpret_cast<const Pack<S, V>*>(src + i * stride + col);
+    for (int u = 0; u < DEEP; ++u) {                      // beyond the end: the first one again, not added
+      i[u] = p + u * Q < b ? p + u * Q : p;
+      if (PERM) i[u] = order[i[u]];
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < DEEP; ++u) x[u] = *reinterpret_cast<const Pack<S, V>*>(src + (int64_t)i[u] * stride + col);
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] += (float)x[u].e[k];
+    for (int u = 0; u < DEEP; ++u)
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += p + u * Q < b ? (float)x[u].e[k] : 0.f;
   }
-  for (; p < e; p += Q) {
-    const int64_t i = PERM ? (int64_t)order[p] : p;
-    const Pack<S, V> x = *reinterpret_cast<const Pack<S, V>*>(src + i * stride + col);
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] += (float)x.e[k];
+}
+
+// acc += one row's positions [a, b), by way of the levels; lane q of Q takes every Q-th entry of each stretch
+template <typename T, int V, int Q, int DEEP>
+__device__ __forceinline__ void grad_row_sum(float (&acc)[V], const T* __restrict__ g, int64_t stride, int64_t at,
+                                             const int32_t* __restrict__ order, int a, int b, int q, int64_t width,
+                                             const GradLevels& lv, const float* __restrict__ sums) {
+  int bits = lv.chunk_bits, level = 0;                       // a, b below 2^31 with room for a block
+  const float* below = sums;                                 // the level's sums, found step by step: an array indexed by
+  int64_t blocks = lv.n[0];                                  // a lane's own level would be copied into registers
+  while (true) {
+    const int up = (a + (1 << bits) - 1) >> bits, down = b >> bits;
+    const bool split = level < lv.count && up < down;        // whole blocks of the next level in the middle
+#pragma unroll 1
+    for (int side = 0; side < (split ? 2 : 1); ++side) {     // one copy of the code: registers decide the speed
+      const int from = side ? down << bits : a, to = split && !side ? up << bits : b;
+      if (level == 0)
+        grad_sum<T, V, true, Q, DEEP>(acc, g, stride, at, order, from + q, to);
+      else
+        grad_sum<float, V, false, Q, DEEP>(acc, below, width, at, nullptr, from + q, to);
+    }
+    if (!split) break;
+    a = up;
+    b = down;
+    bits = lv.fan_bits;
+    if (level) {
+      below += level_space(blocks * width);
+      blocks >>= bits;
+    }
+    ++level;
   }
 }
 
 template <int V, int LE>
-__device__ __forceinline__ void lg_reduce(float (&acc)[V]) {
+__device__ __forceinline__ void grad_join(float (&acc)[V]) {
 #pragma unroll
   for (int off = LE; off < 64; off <<= 1)
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] += __shfl_xor(acc[k], off, 64);
 }
+template <typename O, int V>
+__device__ __forceinline__ void grad_store(O* __restrict__ to, const float (&acc)[V]) {
+  Pack<O, V> o;
+#pragma unroll
+  for (int k = 0; k < V; ++k) o.e[k] = (O)acc[k];
+  *reinterpret_cast<Pack<O, V>*>(to) = o;
+}
 
-// wave b: the sum of sorted positions [b chunk, (b + 1) chunk) if they belong to one row
-template <typename T, int V, int LE>
-__global__ __launch_bounds__(256) void grad_chunk_kernel(const T* __restrict__ g, int64_t stride, int W,
+// One level: block b adds entries [b << bits, (b + 1) << bits) of the level below (the positions themselves for level 1,
+// PERM) if the 1 << span_bits positions that they cover belong to one row.  LE = 0: tc threads per block; else a wave.
+template <typename S, int V, int LE, bool PERM>
+__global__ __launch_bounds__(256) void grad_level_kernel(const S* __restrict__ src, int64_t stride, int W, int tc,
                                                          const int32_t* __restrict__ order,
-                                                         const uint32_t* __restrict__ key, int64_t rows, int64_t n_chunks,
-                                                         int chunk, float* __restrict__ part) {
-  const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (b >= n_chunks) return;
-  const uint32_t k0 = key[b * chunk];
-  if (k0 != key[b * chunk + chunk - 1] || k0 >= rows) return;
-  const int lane = threadIdx.x & 63, q = lane / LE, le = lane % LE;
-  for (int col = le; col - le < W; col += LE) {
+                                                         const uint32_t* __restrict__ key, int64_t rows, int64_t n_blocks,
+                                                         int bits, int span_bits, float* __restrict__ sums) {
+  constexpr int Q = LE ? 64 / (LE ? LE : 1) : 1;
+  const int per = LE ? 4 : 256 / tc, sub = LE ? threadIdx.x >> 6 : threadIdx.x / tc;
+  const int t = LE ? threadIdx.x & 63 : threadIdx.x - sub * tc, step = LE ? LE : tc;
+  const int q = LE ? t / step : 0, col0 = LE ? t % step : t;
+  const int64_t b = (int64_t)blockIdx.x * per + sub;
+  if (sub >= per || b >= n_blocks) return;
+  const uint32_t k0 = key[b << span_bits];
+  if (k0 != key[((b + 1) << span_bits) - 1] || k0 >= rows) return;
+  for (int col = col0; col - col0 < W; col += step) {
     float acc[V] = {};
-    lg_sum<T, V, LE, true>(acc, g, stride, (int64_t)col * V, order, b * chunk, (b + 1) * chunk, q, col < W);
-    lg_reduce<V, LE>(acc);
-    if (q == 0 && col < W)
-#pragma unroll
-      for (int k = 0; k < V; ++k) part[(b * W + col) * V + k] = acc[k];
+    if (col < W)
+      grad_sum<S, V, PERM, Q, LE ? 8 : 4>(acc, src, stride, (int64_t)col * V, order, (int)(b << bits) + q, (int)((b + 1) << bits));
+    if (LE) grad_join<V, LE ? LE : 64>(acc);
+    if (q == 0 && col < W) grad_store<float, V>(sums + (b * W + col) * V, acc);
   }
 }
 
-// wave b: the sum of LG_FAN pure blocks if they belong to one row
-template <int V, int LE>
-__global__ __launch_bounds__(256) void grad_fan_kernel(const float* __restrict__ part, int W,
-                                                       const uint32_t* __restrict__ key, int64_t rows, int64_t n_fans,
-                                                       int chunk, float* __restrict__ part2) {
-  const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (b >= n_fans) return;
-  const int64_t span = (int64_t)chunk * LG_FAN;
-  const uint32_t k0 = key[b * span];
-  if (k0 != key[(b + 1) * span - 1] || k0 >= rows) return;
-  const int lane = threadIdx.x & 63, q = lane / LE, le = lane % LE;
-  for (int col = le; col - le < W; col += LE) {
-    float acc[V] = {};
-    lg_sum<float, V, LE, false>(acc, part, (int64_t)W * V, (int64_t)col * V, nullptr, b * LG_FAN, (b + 1) * LG_FAN, q,
-                                col < W);
-    lg_reduce<V, LE>(acc);
-    if (q == 0 && col < W)
-#pragma unroll
-      for (int k = 0; k < V; ++k) part2[(b * W + col) * V + k] = acc[k];
-  }
-}
-
-template <typename T, int V, int LE, typename O>
-__global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, int64_t stride, int W,
+// A thread per vector; the next row's place in the order is on its way while this one's positions are added.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, int64_t stride, int W, int tc,
                                                        const int32_t* __restrict__ order,
-                                                       const int32_t* __restrict__ start, int64_t rows, int64_t n_chunks,
-                                                       int64_t n_fans, int chunk, const float* __restrict__ part,
-                                                       const float* __restrict__ part2, float scale,
-                                                       O* __restrict__ out) {
-  const int lane = threadIdx.x & 63, q = lane / LE, le = lane % LE;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
-    const int64_t s = start[r], e = start[r + 1];
-    // positions: [s, c0 chunk) and [c1 chunk, e) one by one; pure blocks: [c0, f0 FAN) and [f1 FAN, c1); fans [f0, f1)
-    int64_t c0 = (s + chunk - 1) / chunk, c1 = e / chunk;
-    if (c1 > n_chunks) c1 = n_chunks;
-    const bool split = c0 < c1;
-    int64_t f0 = (c0 + LG_FAN - 1) / LG_FAN, f1 = c1 / LG_FAN;
-    if (f1 > n_fans) f1 = n_fans;
-    const bool fans = split && f0 < f1;
-    for (int col = le; col - le < W; col += LE) {
-      const bool on = col < W;
-      const int64_t at = (int64_t)col * V, ps = (int64_t)W * V;
+                                                       const int32_t* __restrict__ start, int64_t rows, GradLevels lv,
+                                                       const float* __restrict__ sums, float scale, T* __restrict__ out) {
+  const int per_step = 256 / tc, sub = threadIdx.x / tc, col0 = threadIdx.x - sub * tc;
+  int64_t r = (int64_t)blockIdx.x * per_step + sub;
+  if (sub >= per_step || r >= rows) return;
+  const int64_t width = (int64_t)W * V, step = (int64_t)gridDim.x * per_step;
+  int s = start[r], e = start[r + 1];
+  while (true) {
+    const int64_t next = r + step < rows ? r + step : r;
+    const int sn = start[next], en = start[next + 1];
+    for (int col = col0; col < W; col += tc) {
       float acc[V] = {};
-      lg_sum<T, V, LE, true>(acc, g, stride, at, order, s, split ? c0 * chunk : e, q, on);
-      if (split) {
-        lg_sum<float, V, LE, false>(acc, part, ps, at, nullptr, c0, fans ? f0 * LG_FAN : c1, q, on);
-        if (fans) {
-          lg_sum<float, V, LE, false>(acc, part2, ps, at, nullptr, f0, f1, q, on);
-          lg_sum<float, V, LE, false>(acc, part, ps, at, nullptr, f1 * LG_FAN, c1, q, on);
-        }
-        lg_sum<T, V, LE, true>(acc, g, stride, at, order, c1 * chunk, e, q, on);
+      if (e - s == 1) {                                  // most rows of a large table: one position or none
+        const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(g + order[s] * stride + (int64_t)col * V);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = (float)x.e[k] * scale;
+      } else if (e > s) {
+        grad_row_sum<T, V, 1, V == 8 ? 2 : 3>(acc, g, stride, (int64_t)col * V, order, s, e, 0, width, lv, sums);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] *= scale;
       }
-      lg_reduce<V, LE>(acc);
-      if (q == 0 && on) {
-        Pack<O, V> o;
-  #pragma unroll
-        for (int k = 0; k < V; ++k) o.e[k] = (O)(e > s ? acc[k] * scale : 0.f);
-        *reinterpret_cast<Pack<O, V>*>(out + r * ps + at) = o;
+      grad_store<T, V>(out + r * width + (int64_t)col * V, acc);
+    }
+    if (next == r) return;
+    r = next;
+    s = sn;
+    e = en;
+  }
+}
+
+// A wave per row.
+template <typename T, int V, int LE>
+__global__ __launch_bounds__(256) void grad_row_wave_kernel(const T* __restrict__ g, int64_t stride, int W,
+                                                            const int32_t* __restrict__ order,
+                                                            const int32_t* __restrict__ start, int64_t rows, GradLevels lv,
+                                                            const float* __restrict__ sums, float scale,
+                                                            T* __restrict__ out) {
+  const int lane = threadIdx.x & 63, q = lane / LE, le = lane % LE;
+  const int64_t width = (int64_t)W * V;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+    const int s = start[r], e = start[r + 1];
+    for (int col = le; col - le < W; col += LE) {
+      float acc[V] = {};
+      if (col < W)
+        grad_row_sum<T, V, 64 / LE, 4>(acc, g, stride, (int64_t)col * V, order, s, e, q, width, lv, sums);
+      grad_join<V, LE>(acc);
+      if (q == 0 && col < W) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = e > s ? acc[k] * scale : 0.f;
+        grad_store<T, V>(out + r * width + (int64_t)col * V, acc);
       }
+    }
+  }
+}
+
+// Few positions and rows: no sort at all.  A wave per row looks through the ids, 64 at a time, lists the positions it
+// finds in ascending order, and sums them, LE lanes across the columns times 64 / LE over the list.
+constexpr int SCAN_MAX = 2048;
+template <typename T, int V, int LE, typename I>
+__global__ __launch_bounds__(256) void grad_scan_kernel(const T* __restrict__ g, int64_t stride, int W,
+                                                        const I* __restrict__ ids, int n, int64_t rows, float scale,
+                                                        T* __restrict__ out) {
+  constexpr int Q = 64 / LE;
+  __shared__ uint16_t lists[4][SCAN_MAX];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane / LE, le = lane % LE;
+  const int64_t r = (int64_t)blockIdx.x * 4 + wave;
+  uint16_t* list = lists[wave];
+  int found = 0;
+  if (r < rows) {
+    for (int i0 = 0; i0 < n; i0 += 256) {
+      bool hit[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 64 + lane;
+        hit[u] = i < n && (int64_t)ids[i < n ? i : 0] == r;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint64_t m = __ballot(hit[u]);
+        if (hit[u]) list[found + __popcll(m & ((1ull << lane) - 1ull))] = (uint16_t)(i0 + u * 64 + lane);
+        found += __popcll(m);
+      }
+    }
+  }
+  __syncthreads();
+  if (r >= rows) return;
+  for (int col = le; col - le < W; col += LE) {
+    float acc[V] = {};
+    if (col < W) {
+      const T* at = g + (int64_t)col * V;
+      for (int p = q; p < found; p += 4 * Q) {
+        Pack<T, V> x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (p + u * Q < found) x[u] = *reinterpret_cast<const Pack<T, V>*>(at + (int64_t)list[p + u * Q] * stride);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (p + u * Q < found)
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += (float)x[u].e[k];
+      }
+    }
+    grad_join<V, LE>(acc);
+    if (q == 0 && col < W) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] = found ? acc[k] * scale : 0.f;
+      grad_store<T, V>(out + (r * W + col) * V, acc);
     }
   }
 }
@@ -363,17 +585,74 @@ int launch_lookup_v(int v, const void* table, int64_t rows, int64_t width, int64
 
 // ---- the plan's and the scratch's layout, in 4-byte words, 64 words aligned ----
 int64_t words(int64_t n) { return (n + 63) / 64 * 64; }
+
+struct SortShape {
+  int rounds, n_blocks, passes, bits;
+};
+SortShape sort_shape(int64_t rows, int64_t n) {
+  SortShape t;
+  t.rounds = n <= 131072 ? 4 : 16;
+  t.n_blocks = bvi_ceil_div(n, 256 * t.rounds);
+  int bits = 1;
+  while (bits < 32 && ((uint64_t)rows >> bits)) ++bits;                // keys go up to `rows` (padding)
+  t.passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
+  t.bits = (bits + t.passes - 1) / t.passes;
+  return t;
+}
 struct SortScratch {
   int64_t key, val, count, total, all;
 };
-SortScratch sort_scratch(int64_t n) {
-  SortScratch t;
-  t.key = 0;
+SortScratch sort_scratch(int64_t rows, int64_t n) {
+  SortScratch t = {};
+  if (n <= RANK_MAX) return t;
+  const SortShape h = sort_shape(rows, n);
   t.val = words(n);
   t.count = 2 * words(n);
-  t.total = t.count + words((int64_t)RS_DIGITS * bvi_ceil_div(n, RS_TILE));
-  t.all = t.total + RS_DIGITS;
+  t.total = t.count + words((int64_t)h.n_blocks << h.bits);
+  t.all = t.total + words((int64_t)1 << h.bits);
   return t;
+}
+
+template <typename I, int ROUNDS, bool FUSED>
+void launch_scatter(const SortShape& h, const I* ids, const uint32_t* k_in, const uint32_t* v_in, int64_t n, int64_t rows,
+                    int shift, const uint32_t* count, const uint32_t* total, uint32_t* k_out, uint32_t* v_out,
+                    hipStream_t s) {
+#define BVI_SCATTER(E)                                                                                                   \
+  hipLaunchKernelGGL((sort_scatter_kernel<I, ROUNDS, FUSED, E>), dim3(h.n_blocks), dim3(256), 0, s, ids, k_in, v_in, n, \
+                     rows, shift, h.bits, h.n_blocks, count, total, k_out, v_out)
+  if (h.bits == 11) BVI_SCATTER(8);
+  else if (h.bits == 10) BVI_SCATTER(4);
+  else if (h.bits == 9) BVI_SCATTER(2);
+  else BVI_SCATTER(1);
+#undef BVI_SCATTER
+}
+
+template <typename I, int ROUNDS>
+void launch_sort(const I* ids, int64_t n, int64_t rows, uint32_t* order, uint32_t* key, uint32_t* ws, hipStream_t s) {
+  const SortScratch t = sort_scratch(rows, n);
+  const SortShape h = sort_shape(rows, n);
+  const uint32_t* k_in = nullptr;
+  const uint32_t* v_in = nullptr;
+  const int digits = 1 << h.bits;
+  uint32_t *count = ws + t.count, *total = ws + t.total;
+  for (int p = 0; p < h.passes; ++p) {
+    const bool to_plan = ((h.passes - 1 - p) & 1) == 0;                 // the last pass writes the plan
+    uint32_t* k_out = to_plan ? key : ws + t.key;
+    uint32_t* v_out = to_plan ? order : ws + t.val;
+    const int shift = p * h.bits;
+    if (h.n_blocks <= SORT_FUSED) {
+      hipLaunchKernelGGL((sort_count_kernel<I, ROUNDS>), dim3(h.n_blocks), dim3(256), 0, s, ids, k_in, n, rows, shift,
+                         digits, (int64_t)1, (int64_t)digits, count);
+      launch_scatter<I, ROUNDS, true>(h, ids, k_in, v_in, n, rows, shift, count, total, k_out, v_out, s);
+    } else {
+      hipLaunchKernelGGL((sort_count_kernel<I, ROUNDS>), dim3(h.n_blocks), dim3(256), 0, s, ids, k_in, n, rows, shift,
+                         digits, (int64_t)h.n_blocks, (int64_t)1, count);
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), dim3(256), 0, s, h.n_blocks, count, total);
+      launch_scatter<I, ROUNDS, false>(h, ids, k_in, v_in, n, rows, shift, count, total, k_out, v_out, s);
+    }
+    k_in = k_out;
+    v_in = v_out;
+  }
 }
 
 template <typename I>
@@ -381,89 +660,147 @@ int launch_plan(const I* ids, int64_t n, int64_t rows, uint32_t* plan, uint32_t*
   uint32_t* order = plan;
   uint32_t* key = plan + words(n);
   int32_t* start = (int32_t*)(plan + 2 * words(n));
-  if (n > 0) {
-    const SortScratch t = sort_scratch(n);
-    const int n_blocks = bvi_ceil_div(n, RS_TILE);
-    int bits = 1;
-    while (bits < 32 && ((uint64_t)rows >> bits)) ++bits;              // keys go up to `rows` (padding)
-    const int passes = (bits + 7) / 8, per = (bits + passes - 1) / passes;
-    const uint32_t* k_in = nullptr;
-    const uint32_t* v_in = nullptr;
-    for (int p = 0; p < passes; ++p) {
-      const bool to_plan = ((passes - 1 - p) & 1) == 0;                 // the last pass writes the plan
-      uint32_t* k_out = to_plan ? key : ws + t.key;
-      uint32_t* v_out = to_plan ? order : ws + t.val;
-      const uint32_t mask = (1u << per) - 1u;
-      hipLaunchKernelGGL((sort_count_kernel<I>), dim3(n_blocks), dim3(RS_THREADS), 0, s, ids, k_in, n, rows, p * per,
-                         mask, n_blocks, ws + t.count);
-      hipLaunchKernelGGL(sort_scan_kernel, dim3(RS_DIGITS), dim3(256), 0, s, n_blocks, ws + t.count, ws + t.total);
-      hipLaunchKernelGGL((sort_scatter_kernel<I>), dim3(n_blocks), dim3(RS_THREADS), 0, s, ids, k_in, v_in, n, rows,
-                         p * per, mask, n_blocks, ws + t.count, ws + t.total, k_out, v_out);
-      k_in = k_out;
-      v_in = v_out;
-    }
-  }
-  hipLaunchKernelGGL(sort_start_kernel, dim3((unsigned)((rows + 256) / 256)), dim3(256), 0, s, key, n, rows, start);
+  if (n > 0 && n <= RANK_MAX)
+    hipLaunchKernelGGL((sort_rank_kernel<I>), dim3(bvi_ceil_div(n, 32)), dim3(256), 0, s, ids, (int)n, rows, order, key);
+  else if (n > 0 && sort_shape(rows, n).rounds == 4)
+    launch_sort<I, 4>(ids, n, rows, order, key, ws, s);
+  else if (n > 0)
+    launch_sort<I, 16>(ids, n, rows, order, key, ws, s);
+  if (n >= rows)
+    hipLaunchKernelGGL(sort_fill_start_kernel, dim3((unsigned)((n + 256) / 256)), dim3(256), 0, s, key, n, (uint32_t)rows,
+                       start);
+  else
+    hipLaunchKernelGGL(sort_start_kernel, dim3((unsigned)((rows + 256) / 256)), dim3(256), 0, s, key, (int)n, rows, start);
   BVI_HIP_CHECK_LAUNCH();
   return BVI_OK;
 }
+int launch_plan_of(const void* ids, int ids_type, int64_t n, int64_t rows, void* plan, void* ws, hipStream_t s) {
+  if (ids_type == BVI_IDS_I32) return launch_plan((const int32_t*)ids, n, rows, (uint32_t*)plan, (uint32_t*)ws, s);
+  return launch_plan((const int64_t*)ids, n, rows, (uint32_t*)plan, (uint32_t*)ws, s);
+}
+int64_t plan_words(int64_t rows, int64_t n) { return 2 * words(n) + words(rows + 1); }
 
-// positions per pure block: a few vectors per lane, more where that would make very many blocks
-int64_t grad_chunk(int64_t n) { return n >= (1 << 22) ? 512 : 128; }
-int64_t grad_chunks(int64_t n) { return n / grad_chunk(n); }
-int64_t grad_fans(int64_t n) { return grad_chunks(n) >= 4 * LG_FAN ? grad_chunks(n) / LG_FAN : 0; }
-
-template <typename T, int V, int LE, typename O>
-int launch_grad(const void* grad_out, int64_t stride, int64_t n, int64_t width, const uint32_t* plan, int64_t rows,
-                float scale, void* grad_table, float* ws, hipStream_t s) {
-  const int32_t* order = (const int32_t*)plan;
-  const uint32_t* key = plan + words(n);
-  const int32_t* start = (const int32_t*)(plan + 2 * words(n));
-  const int W = (int)(width / V), chunk = (int)grad_chunk(n);
-  const int64_t n_chunks = grad_chunks(n), n_fans = grad_fans(n);
-  float* part = ws;
-  float* part2 = ws + words(n_chunks * width);
-  if (n_chunks > 0) {
-    hipLaunchKernelGGL((grad_chunk_kernel<T, V, LE>), dim3(bvi_ceil_div(n_chunks, 4)), dim3(256), 0, s,
-                       (const T*)grad_out, stride, W, order, key, rows, n_chunks, chunk, part);
-    if (n_fans > 0)
-      hipLaunchKernelGGL((grad_fan_kernel<V, LE>), dim3(bvi_ceil_div(n_fans, 4)), dim3(256), 0, s, part, W, key, rows,
-                         n_fans, chunk, part2);
+// whether a wave sums a row (else threads do): rows of few vectors that have several positions each.  The vectors of a
+// row are counted at their widest, so that the address of an operand does not change the order of the sums.
+bool grad_by_wave(int64_t rows, int64_t width, int64_t n, int size) {
+  int v = 16 / size;
+  while (v > 1 && width % v) v >>= 1;
+  return width / v <= 16 && n >= 4 * rows;
+}
+// the levels of block sums: another one wherever a row could be left with many entries of the one below
+GradLevels grad_levels(int64_t n, int64_t width, bool wave) {
+  GradLevels t;
+  t.count = 0;
+  t.n[0] = 0;
+  t.chunk_bits = wave ? 7 : 4;
+  t.fan_bits = wave ? 6 : 4;
+  int64_t at = 0, m = n >> t.chunk_bits;
+  while (t.count < GRAD_LEVELS && m >= 4) {
+    t.n[t.count] = m;
+    t.at[t.count] = at;
+    at += level_space(m * width);
+    ++t.count;
+    m >>= t.fan_bits;
   }
-  hipLaunchKernelGGL((grad_row_kernel<T, V, LE, O>), dim3((unsigned)((rows + 3) / 4 < (1 << 23) ? (rows + 3) / 4 : (1 << 23))),
-                     dim3(256), 0, s, (const T*)grad_out, stride, W, order, start, rows, n_chunks, n_fans, chunk, part, part2, scale,
-                     (O*)grad_table);
+  return t;
+}
+int64_t level_words(int64_t n, int64_t width, bool wave) {
+  const GradLevels t = grad_levels(n, width, wave);
+  return t.count ? t.at[t.count - 1] + level_space(t.n[t.count - 1] * width) : 0;
+}
+// whether looking through all ids for every row is the quickest way
+bool grad_by_scan(int64_t rows, int64_t n) { return n <= SCAN_MAX && rows * n <= (1 << 22); }
+
+struct GradCall {
+  const void* g;
+  int64_t stride, n, width;
+  const void* ids;
+  int ids_type;
+  bool scan;
+  const uint32_t* plan;
+  int64_t rows;
+  float scale;
+  void* out;
+  float* ws;
+  hipStream_t s;
+};
+
+// LE = 0: threads
+template <typename T, int V, int LE>
+int launch_grad(const GradCall& c) {
+  const int32_t* order = (const int32_t*)c.plan;
+  const uint32_t* key = c.plan + words(c.n);
+  const int32_t* start = (const int32_t*)(c.plan + 2 * words(c.n));
+  const int W = (int)(c.width / V), parts = bvi_ceil_div(W, 256), tc = bvi_ceil_div(W, parts), per = LE ? 4 : 256 / tc;
+  const GradLevels lv = grad_levels(c.n, c.width, LE != 0);
+  int span_bits = 0;
+  for (int l = 0; l < lv.count; ++l) {
+    const int bits = l == 0 ? lv.chunk_bits : lv.fan_bits;
+    const unsigned blocks = (unsigned)((lv.n[l] + per - 1) / per);
+    span_bits += bits;
+    if (l == 0)
+      hipLaunchKernelGGL((grad_level_kernel<T, V, LE, true>), dim3(blocks), dim3(256), 0, c.s, (const T*)c.g, c.stride, W,
+                         tc, order, key, c.rows, lv.n[0], bits, span_bits, c.ws);
+    else
+      hipLaunchKernelGGL((grad_level_kernel<float, V, LE, false>), dim3(blocks), dim3(256), 0, c.s, c.ws + lv.at[l - 1],
+                         c.width, W, tc, order, key, c.rows, lv.n[l], bits, span_bits, c.ws + lv.at[l]);
+  }
+  if (LE) {
+    const int64_t blocks = (c.rows + 3) / 4;
+    hipLaunchKernelGGL((grad_row_wave_kernel<T, V, LE ? LE : 1>), dim3((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22))),
+                       dim3(256), 0, c.s, (const T*)c.g, c.stride, W, order, start, c.rows, lv, c.ws, c.scale, (T*)c.out);
+  } else {
+    const int64_t blocks = (c.rows + per - 1) / per;
+    hipLaunchKernelGGL((grad_row_kernel<T, V>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, c.s,
+                       (const T*)c.g, c.stride, W, tc, order, start, c.rows, lv, c.ws, c.scale, (T*)c.out);
+  }
   BVI_HIP_CHECK_LAUNCH();
   return BVI_OK;
 }
+template <typename T, int V>
+int launch_grad_le(const GradCall& c) {
+  if (!grad_by_wave(c.rows, c.width, c.n, (int)sizeof(T))) return launch_grad<T, V, 0>(c);
+  const int64_t W = c.width / V;
+  if (W > 8) return launch_grad<T, V, 16>(c);
+  if (W > 4) return launch_grad<T, V, 8>(c);
+  if (W > 2) return launch_grad<T, V, 4>(c);
+  if (W > 1) return launch_grad<T, V, 2>(c);
+  return launch_grad<T, V, 1>(c);
+}
 
-template <typename T, int V, typename O>
-int launch_grad_le(const void* g, int64_t stride, int64_t n, int64_t width, const uint32_t* plan, int64_t rows,
-                   float scale, void* out, float* ws, hipStream_t s) {
-  // lanes across the columns: the most that leave at most an eighth of the lanes without a column
-  const int W = (int)(width / V);
-  int le = 64;
-  while (le > 1 && (int64_t)bvi_ceil_div(W, le) * le * 7 > (int64_t)W * 8) le >>= 1;
-  switch (le) {
-    case 64: return launch_grad<T, V, 64, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 32: return launch_grad<T, V, 32, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 16: return launch_grad<T, V, 16, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 8: return launch_grad<T, V, 8, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 4: return launch_grad<T, V, 4, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 2: return launch_grad<T, V, 2, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    default: return launch_grad<T, V, 1, O>(g, stride, n, width, plan, rows, scale, out, ws, s);
-  }
+template <typename T, int V, int LE>
+int launch_scan_le(const GradCall& c) {
+  const dim3 grid((unsigned)((c.rows + 3) / 4));
+  const int W = (int)(c.width / V);
+  if (c.ids_type == BVI_IDS_I32)
+    hipLaunchKernelGGL((grad_scan_kernel<T, V, LE, int32_t>), grid, dim3(256), 0, c.s, (const T*)c.g, c.stride, W,
+                       (const int32_t*)c.ids, (int)c.n, c.rows, c.scale, (T*)c.out);
+  else
+    hipLaunchKernelGGL((grad_scan_kernel<T, V, LE, int64_t>), grid, dim3(256), 0, c.s, (const T*)c.g, c.stride, W,
+                       (const int64_t*)c.ids, (int)c.n, c.rows, c.scale, (T*)c.out);
+  BVI_HIP_CHECK_LAUNCH();
+  return BVI_OK;
+}
+template <typename T, int V>
+int launch_scan(const GradCall& c) {
+  const int64_t W = c.width / V;
+  if (W >= 48) return launch_scan_le<T, V, 64>(c);
+  if (W >= 6) return launch_scan_le<T, V, 16>(c);
+  if (W >= 2) return launch_scan_le<T, V, 4>(c);
+  return launch_scan_le<T, V, 1>(c);
 }
 
 template <typename T>
-int launch_grad_v(const void* g, int64_t stride, int64_t n, int64_t width, const uint32_t* plan, int64_t rows,
-                  float scale, void* out, float* ws, hipStream_t s) {
-  switch (vector_elements(width, stride, (int)sizeof(T), g, out)) {
-    case 8: if constexpr (sizeof(T) == 2) return launch_grad_le<T, 8, T>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 4: return launch_grad_le<T, 4, T>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    case 2: return launch_grad_le<T, 2, T>(g, stride, n, width, plan, rows, scale, out, ws, s);
-    default: return launch_grad_le<T, 1, T>(g, stride, n, width, plan, rows, scale, out, ws, s);
+int launch_grad_v(const GradCall& c) {
+  const int v = vector_elements(c.width, c.stride, (int)sizeof(T), c.g, c.out);
+#define BVI_GRAD_CALL(X) return c.scan ? launch_scan<T, X>(c) : launch_grad_le<T, X>(c)
+  switch (v) {
+    case 8: if constexpr (sizeof(T) == 2) BVI_GRAD_CALL(8);
+    case 4: BVI_GRAD_CALL(4);
+    case 2: BVI_GRAD_CALL(2);
+    default: BVI_GRAD_CALL(1);
   }
+#undef BVI_GRAD_CALL
 }
 
 bool sizes_ok(int64_t rows, int64_t n) {
@@ -496,8 +833,8 @@ int bvi_lookup(const void* table, int dtype, int64_t rows, int64_t width, int64_
 int bvi_lookup_plan_bytes(int64_t rows, int64_t n, size_t* plan_bytes, size_t* ws_bytes) {
   if (!plan_bytes || !ws_bytes || rows < 1 || n < 0) return BVI_ERR_ARG;
   if (!sizes_ok(rows, n)) return BVI_ERR_UNSUPPORTED;
-  *plan_bytes = 4 * (size_t)(2 * words(n) + words(rows + 1));
-  *ws_bytes = 4 * (size_t)sort_scratch(n).all;
+  *plan_bytes = 4 * (size_t)plan_words(rows, n);
+  *ws_bytes = 4 * (size_t)sort_scratch(rows, n).all;
   return BVI_OK;
 }
 
@@ -507,35 +844,45 @@ int bvi_lookup_plan(const void* ids, int ids_type, int64_t n, int64_t rows, void
   if (!sizes_ok(rows, n)) return BVI_ERR_UNSUPPORTED;
   size_t need, scratch;
   bvi_lookup_plan_bytes(rows, n, &need, &scratch);
-  if (!plan || plan_bytes < need || (n > 0 && (!ws || ws_bytes < scratch))) return BVI_ERR_WORKSPACE;
-  if (ids_type == BVI_IDS_I32)
-    return launch_plan((const int32_t*)ids, n, rows, (uint32_t*)plan, (uint32_t*)ws, (hipStream_t)stream);
-  return launch_plan((const int64_t*)ids, n, rows, (uint32_t*)plan, (uint32_t*)ws, (hipStream_t)stream);
+  if (!plan || plan_bytes < need || (scratch && (!ws || ws_bytes < scratch))) return BVI_ERR_WORKSPACE;
+  return launch_plan_of(ids, ids_type, n, rows, plan, ws, (hipStream_t)stream);
 }
 
-int bvi_lookup_grad_ws_bytes(int64_t rows, int64_t width, int64_t n, size_t* ws_bytes) {
+// workspace: the level sums, and without a plan the call's own plan and its sort's scratch
+int bvi_lookup_grad_ws_bytes(int64_t rows, int64_t width, int64_t n, int has_plan, size_t* ws_bytes) {
   if (!ws_bytes || rows < 1 || width < 1 || n < 0) return BVI_ERR_ARG;
   if (!sizes_ok(rows, n) || width > BVI_LOOKUP_MAX) return BVI_ERR_UNSUPPORTED;
-  *ws_bytes = 4 * (size_t)(words(grad_chunks(n) * width) + words(grad_fans(n) * width));
+  *ws_bytes = 0;
+  if (!has_plan && grad_by_scan(rows, n)) return BVI_OK;
+  // the type is not known here: the larger of the two forms' levels
+  const int64_t a = level_words(n, width, false), b = level_words(n, width, true);
+  *ws_bytes = 4 * (size_t)((a > b ? a : b) + (has_plan ? 0 : plan_words(rows, n) + sort_scratch(rows, n).all));
   return BVI_OK;
 }
 
-int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, int64_t row_stride, const void* plan,
-                    int64_t rows, float scale, void* grad_table, void* ws, size_t ws_bytes, void* stream) {
-  if ((!grad_out && n > 0) || !type_size(dtype) || n < 0 || width < 1 || row_stride < width || rows < 1 || !plan ||
-      !grad_table)
+int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, int64_t row_stride, const void* ids,
+                    int ids_type, const void* plan, int64_t rows, float scale, void* grad_table, void* ws,
+                    size_t ws_bytes, void* stream) {
+  if ((!grad_out && n > 0) || !type_size(dtype) || n < 0 || width < 1 || row_stride < width || rows < 1 || !grad_table)
     return BVI_ERR_ARG;
+  if ((!plan && !ids && n > 0) || (ids && (ids_type != BVI_IDS_I32 && ids_type != BVI_IDS_I64))) return BVI_ERR_ARG;
   if (!sizes_ok(rows, n) || width > BVI_LOOKUP_MAX) return BVI_ERR_UNSUPPORTED;
   size_t need;
-  bvi_lookup_grad_ws_bytes(rows, width, n, &need);
+  bvi_lookup_grad_ws_bytes(rows, width, n, plan != nullptr, &need);
   if (need && (!ws || ws_bytes < need)) return BVI_ERR_WORKSPACE;
-  const hipStream_t s = (hipStream_t)stream;
-  const uint32_t* p = (const uint32_t*)plan;
-  if (dtype == BVI_TYPE_F32)
-    return launch_grad_v<float>(grad_out, row_stride, n, width, p, rows, scale, grad_table, (float*)ws, s);
-  if (dtype == BVI_TYPE_BF16)
-    return launch_grad_v<__bf16>(grad_out, row_stride, n, width, p, rows, scale, grad_table, (float*)ws, s);
-  return launch_grad_v<_Float16>(grad_out, row_stride, n, width, p, rows, scale, grad_table, (float*)ws, s);
+  // the same way with and without a plan, so that both give the same bits
+  const bool scan = (ids || n == 0) && grad_by_scan(rows, n);
+  GradCall c{grad_out, row_stride, n, width, ids, ids_type, scan, (const uint32_t*)plan, rows, scale, grad_table,
+             (float*)ws, (hipStream_t)stream};
+  if (!plan && !scan) {
+    uint32_t* own = (uint32_t*)((char*)ws + need) - plan_words(rows, n) - sort_scratch(rows, n).all;
+    const int st = launch_plan_of(ids, ids_type, n, rows, own, own + plan_words(rows, n), c.s);
+    if (st) return st;
+    c.plan = own;
+  }
+  if (dtype == BVI_TYPE_F32) return launch_grad_v<float>(c);
+  if (dtype == BVI_TYPE_BF16) return launch_grad_v<__bf16>(c);
+  return launch_grad_v<_Float16>(c);
 }
 
 }  // extern "C"

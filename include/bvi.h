@@ -472,8 +472,9 @@ int bvi_philox_normal(uint64_t seed, uint64_t step, int n_chains, int n_params, 
  * int64; an id outside [0, rows) is padding: it reads zeros and takes no part in the gradient.
  *   bvi_lookup            out[n, width] = scale * table[ids]; the product in float, rounded once
  *   bvi_lookup_plan       what the gradient needs of the ids alone (a stable sort; int32 order[n], key[n],
- *                         start[rows + 1]): once per dataset, or per call where the ids change
- *   bvi_lookup_grad       grad_table[rows, width] = scale * the sums of grad_out's rows per id, in float, rounded once;
+ *                         start[rows + 1]), for callers whose ids stay the same: once per dataset
+ *   bvi_lookup_grad       from the ids (sorted within the call), from a plan of them (ids may be NULL), or both;
+ *                         grad_table[rows, width] = scale * the sums of grad_out's rows per id, in float, rounded once;
  *                         every row is written (zeros where no id asks for it); no atomics, the same bits every time
  * dtype is that of table, out, grad_out and grad_table.  rows, width and n at most BVI_LOOKUP_MAX. */
 #define BVI_TYPE_F32 0
@@ -487,9 +488,10 @@ int bvi_lookup(const void* table, int dtype, int64_t rows, int64_t width, int64_
 int bvi_lookup_plan_bytes(int64_t rows, int64_t n, size_t* plan_bytes, size_t* ws_bytes);
 int bvi_lookup_plan(const void* ids, int ids_type, int64_t n, int64_t rows, void* plan, size_t plan_bytes, void* ws,
                     size_t ws_bytes, void* stream);
-int bvi_lookup_grad_ws_bytes(int64_t rows, int64_t width, int64_t n, size_t* ws_bytes);
-int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, int64_t row_stride, const void* plan,
-                    int64_t rows, float scale, void* grad_table, void* ws, size_t ws_bytes, void* stream);
+int bvi_lookup_grad_ws_bytes(int64_t rows, int64_t width, int64_t n, int has_plan, size_t* ws_bytes);
+int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, int64_t row_stride, const void* ids,
+                    int ids_type, const void* plan, int64_t rows, float scale, void* grad_table, void* ws,
+                    size_t ws_bytes, void* stream);
 
 /* ---- Gaussian linear regression with group-level effects: the loss that reads such tables, with its gradient.
  *   y_i ~ Normal(b + x_i . w + sum_l z_il u_l[ids_l[i]], s);  theta = (b, w[d], s, u_1[rows_1], u_2[rows_2], ...)

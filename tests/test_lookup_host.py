@@ -60,9 +60,11 @@ def test_c_entry_points_refuse_before_launching():
     assert lib.bvi_lookup_plan_bytes(1 << 31, 5, ctypes.byref(z), ctypes.byref(z)) == -2
     assert lib.bvi_lookup_plan(p, 1, 5, 4, p, 16, p, 16, None) == -3
     assert lib.bvi_lookup_plan(None, 1, 5, 4, p, 1 << 30, p, 1 << 30, None) == -1
-    assert lib.bvi_lookup_grad_ws_bytes(4, 0, 5, ctypes.byref(z)) == -1
-    assert lib.bvi_lookup_grad(p, 0, 5, 3, 3, None, 4, 1.0, p, p, 16, None) == -1
-    assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 4, 1.0, p, None, 0, None) == -3
+    assert lib.bvi_lookup_grad_ws_bytes(4, 0, 5, 0, ctypes.byref(z)) == -1
+    assert lib.bvi_lookup_grad(p, 0, 5, 3, 3, None, 0, None, 4, 1.0, p, p, 16, None) == -1      # neither ids nor a plan
+    assert lib.bvi_lookup_grad(p, 0, 5, 3, 3, p, 5, None, 4, 1.0, p, p, 16, None) == -1
+    assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 0, p, 4, 1.0, p, None, 0, None) == -3
+    assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 0, None, 4, 1.0, p, p, 16, None) == -3
     ptrs, types = (ctypes.c_void_p * 1)(4096), (ctypes.c_int * 1)(0)
     assert lib.bvi_global_norm(0, ptrs, one, types, p, p, 1 << 20, None) == -1
     assert lib.bvi_global_norm(1, ptrs, one, (ctypes.c_int * 1)(9), p, p, 1 << 20, None) == -1
