@@ -247,8 +247,7 @@ def _own(s):
 
 def run(state):
     if own:
-        _package()
-        return _own(state)
+        return _own(state)                 # the package's path was set when prepare() made what the program keeps
     return {'lookup': _plain_lookup, 'gradient': _plain_gradient, 'clip': _plain_clip, 'adam': _plain_adam,
             'regression': _plain_regression}[state['kind']](state)
 
