@@ -177,7 +177,7 @@ def _ptr(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _check_f32_cuda(*ts):
@@ -403,15 +403,16 @@ def mvn_tril_logp_grad(Y, theta, parameterisation, ws: Workspace, want_grad=True
 
 # ---- lookups, grouped regression, lists of tensors ----
 class _Here:
-    """Makes a tensor's device the current one for a call (most calls find it so)."""
+    """Makes a tensor's device the current one for a call (most calls find it so); gives its current stream."""
 
     def __init__(self, device):
+        self.index = device.index
         self.other = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.other is not None:
             self.other.__enter__()
-        return _stream()
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.other is not None:
@@ -452,7 +453,7 @@ def lookup_grad(g, n, width, row_stride, ids, plan, rows, scale, out):
 
 
 def _pointers(ts):
-    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() if t is not None else None for t in ts])
+    return (ctypes.c_void_p * len(ts))(*[None if t is None else t.data_ptr() for t in ts])
 
 
 def _int64s(values):
@@ -482,9 +483,8 @@ def grouped_ws_bytes(n, d, rows, n_chains):
     return int(a.value)
 
 
-def _tensor_list(tensors, what):
-    if not isinstance(tensors, (list, tuple)) or not tensors:
-        raise TypeError('%s takes a non-empty list of tensors' % what)
+def tensor_list(tensors, what):
+    """The device of a list of GPU tensors of the types the kernels take; raises otherwise."""
     device = None
     for t in tensors:
         if not isinstance(t, torch.Tensor) or t.dtype not in ELEMENT_TYPES:
@@ -492,10 +492,23 @@ def _tensor_list(tensors, what):
                             % (what, t.dtype if isinstance(t, torch.Tensor) else type(t).__name__))
         if not t.is_cuda:
             raise BviError('%s: tensors must be on the GPU (there is no CPU fallback); got %s' % (what, t.device))
-        if device is not None and t.device != device:
-            raise ValueError('%s: tensors on %s and on %s' % (what, device, t.device))
-        device = t.device
+        d = t.device
+        if device is not None and d != device:
+            raise ValueError('%s: tensors on %s and on %s' % (what, device, d))
+        device = d
     return device
+
+
+_NORM_WS = {}
+
+
+def _norm_scratch(n, device):
+    nbytes = _NORM_WS.get(n)
+    if nbytes is None:
+        a = ctypes.c_size_t(0)
+        check(lib().bvi_global_norm_ws_bytes(n, ctypes.byref(a)), 'bvi_global_norm_ws_bytes')
+        nbytes = _NORM_WS[n] = int(a.value)
+    return _scratch(nbytes, device)
 
 
 def _list_arguments(tensors):
@@ -504,15 +517,8 @@ def _list_arguments(tensors):
             (ctypes.c_int * n)(*[ELEMENT_TYPES[t.dtype] for t in tensors]))
 
 
-def _norm_scratch(n, device):
-    a = ctypes.c_size_t(0)
-    check(lib().bvi_global_norm_ws_bytes(n, ctypes.byref(a)), 'bvi_global_norm_ws_bytes')
-    return _scratch(a.value, device)
-
-
-def global_norm(tensors):
-    """bvi_global_norm of contiguous tensors: a float32 scalar on their device."""
-    device = _tensor_list(tensors, 'global_norm')
+def global_norm(tensors, device):
+    """bvi_global_norm of contiguous tensors that `tensor_list` accepted: a float32 scalar on their device."""
     with _Here(device) as st:
         n, ptrs, sizes, types = _list_arguments(tensors)
         norm, ws = torch.empty((), dtype=torch.float32, device=device), _norm_scratch(n, device)
@@ -521,17 +527,16 @@ def global_norm(tensors):
     return norm
 
 
-def clip_by_global_norm(tensors, outputs, clip_norm, use_norm=None):
-    """bvi_clip_by_global_norm of contiguous tensors into `outputs` (same shapes and types; may be the tensors
-    themselves); returns the norm."""
-    device = _tensor_list(tensors, 'clip_by_global_norm')
+def clip_by_global_norm(tensors, outputs, clip_norm, use_norm, device):
+    """bvi_clip_by_global_norm of contiguous tensors that `tensor_list` accepted into `outputs` (same shapes and types;
+    may be the tensors themselves); returns the norm."""
     with _Here(device) as st:
         n, ptrs, sizes, types = _list_arguments(tensors)
         norm = torch.empty((), dtype=torch.float32, device=device)
-        ws = _norm_scratch(n, device) if use_norm is None else None
-        check(lib().bvi_clip_by_global_norm(n, ptrs, _pointers(outputs), sizes, types, clip_norm, _ptr(use_norm),
-                                            norm.data_ptr(), _ptr(ws), ws.numel() if ws is not None else 0, st),
-              'bvi_clip_by_global_norm')
+        ws = _norm_scratch(n, device)
+        check(lib().bvi_clip_by_global_norm(n, ptrs, ptrs if outputs is tensors else _pointers(outputs), sizes, types,
+                                            clip_norm, None if use_norm is None else use_norm.data_ptr(), norm.data_ptr(),
+                                            ws.data_ptr(), ws.numel(), st), 'bvi_clip_by_global_norm')
     return norm
 
 

@@ -67,26 +67,26 @@ class _AdamState:
         one launch of bvi_clip_adam_step (norm, clip, moments, update) instead of some seven element-wise kernels,
         which is most of a step's launches for a flow with a few dozen small variables.  With `global_clipnorm`, or a
         variable too large for one workgroup, all variables go through bvi_adam_step together."""
-        live = [(p, m, v) for p, m, v in zip(self.params, self.m, self.v) if p.grad is not None]
+        live = [(p, g, m, v) for p, g, m, v in zip(self.params, [p.grad for p in self.params], self.m, self.v)
+                if g is not None]
         on_device = bool(live) and all(p.is_cuda and p.dtype == torch.float32 and p.is_contiguous()
-                                       and p.grad.is_contiguous() and p.grad.dtype == torch.float32 for p, _, _ in live)
+                                       and g.is_contiguous() and g.dtype == torch.float32 for p, g, _, _ in live)
         if not on_device:
             with torch.no_grad():
-                for p, _, _ in live:     # without a host sync
-                    p.grad.mul_(torch.clamp(clip_norm / (p.grad.norm() + 1e-30), max=1.0))
+                for _, g, _, _ in live:     # without a host sync
+                    g.mul_(torch.clamp(clip_norm / (g.norm() + 1e-30), max=1.0))
             self.step()
             return
-        if self.global_clipnorm is not None or any(p.numel() > ONE_WORKGROUP_MAX for p, _, _ in live):
+        if self.global_clipnorm is not None or any(p.numel() > ONE_WORKGROUP_MAX for p, _, _, _ in live):
             hyper = (self.lr, self.b1, self.b2, self.eps)
             if self.global_clipnorm is None:      # the constants that bvi_clip_adam_step takes: same results to rounding
                 hyper = tuple(float(np.float32(h)) for h in hyper)
-            _native.adam_step([p.detach() for p, _, _ in live], [p.grad for p, _, _ in live], [m for _, m, _ in live],
-                              [v for _, _, v in live], self.t, *hyper, float(clip_norm), self.global_clipnorm or 0.0)
+            _native.adam_step(*zip(*live), self.t, *hyper, float(clip_norm), self.global_clipnorm or 0.0)
             return
         lib, ptr, st = _native.lib(), _native._ptr, _native._stream()
         with torch.no_grad():
-            for i, (p, m, v) in enumerate(live):
-                _native.check(lib.bvi_clip_adam_step(p.numel(), ptr(p), ptr(p.grad), ptr(m), ptr(v), ptr(self.t),
+            for i, (p, g, m, v) in enumerate(live):
+                _native.check(lib.bvi_clip_adam_step(p.numel(), ptr(p), ptr(g), ptr(m), ptr(v), ptr(self.t),
                                                      1 if i == 0 else 0, self.lr, self.b1, self.b2, self.eps,
                                                      float(clip_norm), st), 'bvi_clip_adam_step')
 

@@ -41,17 +41,18 @@ def cholesky_solve(chol, rhs):
 def _listed(t_list, what):
     if not isinstance(t_list, (list, tuple)):
         raise TypeError('%s takes a list of tensors, got %s' % (what, type(t_list).__name__))
-    live = [t.detach() if isinstance(t, torch.Tensor) else t for t in t_list if t is not None]
+    live = [t for t in t_list if t is not None]
     if not live:
         raise ValueError('%s: no tensor in the list' % what)
-    _native._tensor_list(live, what)
-    return live
+    return live, _native.tensor_list(live, what)
 
 
 def global_norm(t_list):
     """tf.linalg.global_norm: sqrt of the sum of all squares of a list of GPU tensors (float32, bfloat16, float16, mixed;
     None entries are skipped), a float32 scalar on the device.  Squares are summed in double.  Not differentiable."""
-    return _native.global_norm([t.contiguous() for t in _listed(t_list, 'global_norm')])
+    live, device = _listed(t_list, 'global_norm')
+    with torch.no_grad():
+        return _native.global_norm([t.contiguous() for t in live], device)
 
 
 def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
@@ -60,15 +61,14 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
     every entry becomes NaN, as in tf.  None entries stay None.  `inplace=True` writes the tensors themselves (contiguous
     ones, no two of them overlapping) and returns them; nothing is written where nothing has to be clipped.  Nothing
     synchronises.  Not differentiable."""
-    live = _listed(t_list, 'clip_by_global_norm')
+    live, device = _listed(t_list, 'clip_by_global_norm')
     clip_norm = float(clip_norm)
     if not clip_norm > 0.0:
         raise ValueError('clip_norm must be positive, got %r' % clip_norm)
     if use_norm is not None:
         if not (isinstance(use_norm, torch.Tensor) and use_norm.dtype == torch.float32 and use_norm.numel() == 1
-                and use_norm.device == live[0].device):
-            raise ValueError('use_norm must be one float32 on %s' % live[0].device)
-        use_norm = use_norm.detach()
+                and use_norm.device == device):
+            raise ValueError('use_norm must be one float32 on %s' % device)
     if inplace:
         if not all(t.is_contiguous() for t in live):
             raise ValueError('clip_by_global_norm(inplace=True) needs contiguous tensors')
@@ -77,8 +77,13 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
             raise ValueError('clip_by_global_norm(inplace=True): two tensors of the list overlap')
         src = out = live
     else:
-        src = [t.contiguous() for t in live]
-        out = [torch.empty_like(t) for t in src]
-    norm = _native.clip_by_global_norm(src, out, clip_norm, use_norm)
+        with torch.no_grad():
+            src = [t.contiguous() for t in live]
+            out = [torch.empty_like(t) for t in src]
+    norm = _native.clip_by_global_norm(src, out, clip_norm, use_norm, device)
+    if inplace:
+        return list(t_list), norm
+    if len(live) == len(t_list):
+        return out, norm
     result = iter(out)
-    return [None if t is None else (t if inplace else next(result)) for t in t_list], norm
+    return [None if t is None else next(result) for t in t_list], norm
