@@ -33,14 +33,18 @@ struct GrPass {                         // one lookup's copy of the rows
   int own, lookups;
 };
 
-// CP chains x 64 / CP rows per wave.  FIRST: this pass also takes the sums that need every row once.
+// CP chains x 64 / CP rows per wave.  FIRST: this pass also takes the sums that need every row once.  With 64 chains a
+// wave's rows are the same for all lanes: y, X and the group come through scalar loads, and a row costs 2 D + 3 vector
+// instructions (hence the pointers of their own: the compiler must see that nothing here writes what they point to).
 template <int CP, int D, bool GRAD, bool FIRST>
-__global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPass a, int64_t n, int d, int64_t span, int C, int64_t P,
-                                                                const float* __restrict__ theta,
-                                                                const float* __restrict__ tables,
-                                                                float* __restrict__ slots, double* __restrict__ dense) {
+__global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
+    GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
+    const float* __restrict__ zown, const int32_t* __restrict__ start, int64_t n, int d, int64_t span, int C, int64_t P,
+    const float* __restrict__ theta, const float* __restrict__ tables, float* __restrict__ slots,
+    double* __restrict__ dense) {
   constexpr int Q = 64 / CP;
   constexpr int DD = D ? D : 1;
+  constexpr int U = D <= 16 ? 4 : 1;                       // rows in flight
   const int lane = threadIdx.x & 63, cl = lane % CP, q = lane / CP;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chain = blockIdx.y * CP + cl;
@@ -56,26 +60,21 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPass a, int64_
   }
   double sum_e = 0.0, sum_sq = 0.0;
   const int own = a.own;
-  const int32_t* key = a.id[own];
-  const float* zown = a.z[own];
+  const int64_t rows = a.rows[own];
   const int64_t wid = (int64_t)blockIdx.x * GR_WAVES + wave;
   int64_t i0 = wid * span;
   const int64_t end = i0 + span < n ? i0 + span : n;
   while (i0 < end) {
-    const int64_t g = key[i0];
-    const bool inside = g >= 0 && g < a.rows[own];
-    int64_t e0 = inside ? (int64_t)a.start[g + 1] : end;
+    const int g = __builtin_amdgcn_readfirstlane(key[i0]);
+    const bool inside = g >= 0 && g < rows;
+    int64_t e0 = inside ? (int64_t)__builtin_amdgcn_readfirstlane(start[g + 1]) : end;
     if (e0 > end) e0 = end;
     const float u = !inside ? 0.f : tables ? tables[(a.at[own] + g) * C + c] : th[a.offset[own] + g];
+    const float base = zown ? b : b + u;
     float se = 0.f, sq = 0.f, su = 0.f;
-    for (int64_t i = i0 + q; i < e0; i += Q) {
-      float x[DD];
-      if (D > 0) {
-#pragma unroll
-        for (int j = 0; j < D; ++j) x[j] = a.X[i * D + j];
-      }
-      const float zo = zown ? zown[i] : 1.f;
-      float r = a.y[i] - b - u * zo;
+    auto row = [&](float yi, const float* x, float zo, int64_t i) {
+      float r = yi - base;
+      if (zown) r = fmaf(-u, zo, r);
       for (int l = 0; l < a.lookups; ++l) {
         if (l == own) continue;
         const int64_t k = a.id[l][i];
@@ -85,52 +84,69 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPass a, int64_
 #pragma unroll
         for (int j = 0; j < D; ++j) r = fmaf(-w[j], x[j], r);
       }
-      if (FIRST) {
-        sq = fmaf(r, r, sq);
-        if (GRAD) {
-          se += r;
-          if (D > 0) {
+      if (FIRST) sq = fmaf(r, r, sq);
+      if (GRAD) se += r;
+      if (GRAD && zown) su = fmaf(r, zo, su);
+      if (FIRST && GRAD && D > 0) {
 #pragma unroll
-            for (int j = 0; j < D; ++j) gw[j] = fmaf(r, x[j], gw[j]);
-          }
-        }
+        for (int j = 0; j < D; ++j) gw[j] = fmaf(r, x[j], gw[j]);
       }
-      if (GRAD) su = fmaf(r, zo, su);
+    };
+    int64_t i = i0 + q;
+    for (; i + (U - 1) * Q < e0; i += U * Q) {
+      float yi[U], zo[U], x[U][DD];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        yi[k] = y[i + k * Q];
+        zo[k] = zown ? zown[i + k * Q] : 1.f;
+#pragma unroll
+        for (int j = 0; j < D; ++j) x[k][j] = X[(i + k * Q) * D + j];
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) row(yi[k], x[k], zo[k], i + k * Q);
+    }
+    for (; i < e0; i += Q) {
+      float x[DD];
+#pragma unroll
+      for (int j = 0; j < D; ++j) x[j] = X[i * D + j];
+      row(y[i], x, zown ? zown[i] : 1.f, i);
     }
     if (FIRST) {
       sum_sq += (double)sq;
       sum_e += (double)se;
     }
     if (GRAD && inside) {
+      float v = zown ? su : se;
 #pragma unroll
-      for (int off = CP; off < 64; off <<= 1) su += __shfl_xor(su, off, 64);
-      if (q == 0 && live) slots[(g + wid) * C + c] = su;
+      for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+      if (q == 0 && live) slots[(g + wid) * C + c] = v;
     }
     i0 = e0;
   }
   if (!FIRST) return;
-  // the workgroup's dense sums: [0] e^2, [1] e, [2 + j] e x_j
-  __shared__ double red[GR_WAVES][CP];
+  // the workgroup's dense sums: [0] e^2, [1] e, [2 + j] e x_j; eight at a time through LDS
+  constexpr int COUNT = GRAD ? 2 + D : 1;
   const int count = GRAD ? 2 + d : 1;
-  for (int k = 0; k < count; ++k) {
-    double v;
-    if (k == 0) v = sum_sq;
-    else if (k == 1) v = sum_e;
-    else {
-      float f = 0.f;
+  __shared__ double red[GR_WAVES][8][CP];
 #pragma unroll
-      for (int j = 0; j < DD; ++j) f = k - 2 == j ? gw[j] : f;
-      v = (double)f;
+  for (int k0 = 0; k0 < COUNT; k0 += 8) {
+    __syncthreads();
+#pragma unroll
+    for (int k = k0; k < k0 + 8 && k < COUNT; ++k) {
+      double v = k == 0 ? sum_sq : k == 1 ? sum_e : (double)gw[k >= 2 ? k - 2 : 0];
+#pragma unroll
+      for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+      if (q == 0) red[wave][k - k0][cl] = v;
     }
+    __syncthreads();
+    for (int t = threadIdx.x; t < 8 * CP; t += 64 * GR_WAVES) {
+      const int k = k0 + t / CP, ch = blockIdx.y * CP + t % CP;
+      if (k < count && ch < C) {
+        double v = 0.0;
 #pragma unroll
-    for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
-    __syncthreads();
-    if (q == 0) red[wave][cl] = v;
-    __syncthreads();
-    if (threadIdx.x < CP && blockIdx.y * CP + threadIdx.x < (unsigned)C) {
-      double t = 0.0;
-      for (int x = 0; x < GR_WAVES; ++x) t += red[x][threadIdx.x];
-      dense[((int64_t)blockIdx.x * count + k) * C + blockIdx.y * CP + threadIdx.x] = t;
+        for (int x = 0; x < GR_WAVES; ++x) v += red[x][t / CP][t % CP];
+        dense[((int64_t)blockIdx.x * count + k) * C + ch] = v;
+      }
     }
   }
 }
@@ -157,9 +173,9 @@ struct GrFinish {
   int lookups;
 };
 
-// Workgroup x < count: dense sum x.  Others: 1024 / CP groups of a table; a thread adds one group's slots for one
-// chain, the workgroup together those of a group with many.
-constexpr int GR_MANY = 64;
+// Workgroup x < count: dense sum x.  Others: 1024 / CP groups of a table.  A thread adds up a group's slots for one chain
+// where they are few, a wave where they are not, the workgroup together where the wave's lanes would be too few.
+constexpr int GR_MANY = 16, GR_VERY_MANY = 512;
 template <int CP>
 __global__ __launch_bounds__(1024) void grouped_finish_kernel(GrFinish f, int64_t n, int d, int count, int64_t span,
                                                               int n_blocks, int C, int64_t P,
@@ -167,24 +183,42 @@ __global__ __launch_bounds__(1024) void grouped_finish_kernel(GrFinish f, int64_
                                                               const double* __restrict__ dense,
                                                               const double* __restrict__ logp_ref,
                                                               float* __restrict__ logp, float* __restrict__ grad) {
-  constexpr int GT = 1024 / CP;
-  __shared__ double red[1024];
+  constexpr int GT = 1024 / CP, Q = 64 / CP;
+  __shared__ double red[1024], val[1024];
   const int cl = threadIdx.x % CP, q = threadIdx.x / CP;
   const int chain = blockIdx.y * CP + cl;
   const int c = chain < C ? chain : C - 1;
   const double s = (double)theta[(int64_t)c * P + 1 + d];
-  if ((int)blockIdx.x < count) {
-    const int k = blockIdx.x;
+  // entries first, first + step, ... below `past` of one chain's column; eight loads in flight
+  auto column = [&](auto* __restrict__ p, int64_t first, int64_t past, int step, int64_t stride) {
     double v = 0.0;
-    for (int x = q; x < n_blocks; x += GT) v += dense[((int64_t)x * count + k) * C + c];
+    for (int64_t k = first; k < past; k += 8 * step) {
+      double x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t at = k + u * step;
+        x[u] = (double)p[(at < past ? at : k) * stride];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += k + u * step < past ? x[u] : 0.0;
+    }
+    return v;
+  };
+  auto block_total = [&](double v) {                             // over q, for every cl
     red[threadIdx.x] = v;
     __syncthreads();
     for (int h = GT / 2; h >= 1; h >>= 1) {
       if (q < h) red[threadIdx.x] += red[threadIdx.x + h * CP];
       __syncthreads();
     }
+    v = red[cl];
+    __syncthreads();
+    return v;
+  };
+  if ((int)blockIdx.x < count) {
+    const int k = blockIdx.x;
+    const double v = block_total(column(dense + (int64_t)k * C + c, q, n_blocks, GT, (int64_t)count * C));
     if (q == 0 && chain < C) {
-      v = red[cl];
       if (k == 0) {
         const double level = logp_ref ? *logp_ref : 0.0;
         logp[c] = (float)(-(double)n * log(s) - 0.5 * (double)n * BVI_LN2PI_D - 0.5 * v / (s * s) - level);
@@ -198,44 +232,50 @@ __global__ __launch_bounds__(1024) void grouped_finish_kernel(GrFinish f, int64_
   const int64_t tile = blockIdx.x - count;
   int l = 0;
   while (l + 1 < f.lookups && tile >= f.tile_end[l]) ++l;
-  const int64_t g0 = (tile - (l ? f.tile_end[l - 1] : 0)) * GT, g = g0 + q, rows = f.rows[l];
+  const int64_t g0 = (tile - (l ? f.tile_end[l - 1] : 0)) * GT, rows = f.rows[l];
   const float* slots = f.slots[l];
-  double v = 0.0;
-  int64_t first = 0, last = -1;
-  if (g < rows) {
-    const int64_t b = f.start[l][g], e = f.start[l][g + 1];
+  const int32_t* start = f.start[l];
+  // slots [first, past) of the tile's group k
+  auto slots_of = [&](int k, int64_t* first, int64_t* past) {
+    *first = *past = 0;
+    if (g0 + k >= rows) return;
+    const int64_t b = start[g0 + k], e = start[g0 + k + 1];
     if (e > b) {
-      first = g + b / span;
-      last = g + (e - 1) / span;
+      *first = g0 + k + b / span;
+      *past = g0 + k + (e - 1) / span + 1;
     }
+  };
+  __shared__ int some[GT], very[GT], n_some, n_very;             // groups left to the waves, to the workgroup
+  if (threadIdx.x == 0) n_some = n_very = 0;
+  __syncthreads();
+  int64_t first, past;
+  slots_of(q, &first, &past);
+  if (past - first <= GR_MANY) {
+    val[threadIdx.x] = column(slots + c, first, past, 1, C);
+  } else if (cl == 0) {
+    // the order of the lists only says who does which group
+    if (past - first <= GR_VERY_MANY) some[atomicAdd(&n_some, 1)] = q;
+    else very[atomicAdd(&n_very, 1)] = q;
   }
-  const bool many = last - first >= GR_MANY;
-  if (!many)
-    for (int64_t k = first; k <= last; ++k) v += (double)slots[k * C + c];
-  // groups with many slots, one after the other by everyone (`many` of a group is the same in its CP threads)
-  __shared__ int queue[GT];
-  __shared__ int queued;
-  if (threadIdx.x == 0) queued = 0;
   __syncthreads();
-  if (many && cl == 0) queue[atomicAdd(&queued, 1)] = q;        // the order only says which goes first
-  __syncthreads();
-  const int waiting = queued;
+  const int lane = threadIdx.x & 63, wq = lane / CP;             // cl is also the lane's chain: CP divides 64
+  for (int x = threadIdx.x >> 6; x < n_some; x += 16) {
+    slots_of(some[x], &first, &past);
+    double v = column(slots + c, first + wq, past, Q, C);
+#pragma unroll
+    for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+    if (wq == 0) val[some[x] * CP + cl] = v;
+  }
+  const int waiting = n_very;
   for (int x = 0; x < waiting; ++x) {
-    const int64_t gg = g0 + queue[x], b = f.start[l][gg], e = f.start[l][gg + 1];
-    double t = 0.0;
-    for (int64_t k = gg + b / span + q; k <= gg + (e - 1) / span; k += GT) t += (double)slots[k * C + c];
-    red[threadIdx.x] = t;
-    __syncthreads();
-    for (int h = GT / 2; h >= 1; h >>= 1) {
-      if (q < h) red[threadIdx.x] += red[threadIdx.x + h * CP];
-      __syncthreads();
-    }
-    if (q == queue[x]) v = red[cl];
-    __syncthreads();
+    slots_of(very[x], &first, &past);
+    const double v = block_total(column(slots + c, first + q, past, GT, C));
+    if (q == 0) val[very[x] * CP + cl] = v;
   }
+  __syncthreads();
   // neighbouring threads write neighbouring groups of one chain
   float* out = reinterpret_cast<float*>(red);
-  out[threadIdx.x] = (float)(v / (s * s));
+  out[threadIdx.x] = (float)(val[threadIdx.x] / (s * s));
   __syncthreads();
   const int wc = threadIdx.x / GT, wg = threadIdx.x % GT;
   if (blockIdx.y * CP + wc < (unsigned)C && g0 + wg < rows)
@@ -342,7 +382,7 @@ template <int CP, int D, bool GRAD, bool FIRST>
 void launch_pass(const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P, const float* theta,
                  const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
   hipLaunchKernelGGL((grouped_kernel<CP, D, GRAD, FIRST>), dim3(blocks, bvi_ceil_div(C, CP)), dim3(64 * GR_WAVES), 0, s, a,
-                     n, d, span, C, P, theta, tables, slots, dense);
+                     a.y, a.X, a.id[a.own], a.z[a.own], a.start, n, d, span, C, P, theta, tables, slots, dense);
 }
 template <int CP, int D>
 void launch_pass_mode(bool grad, bool first, const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P,
