@@ -19,6 +19,7 @@
 namespace {
 
 constexpr int GR_WAVES = 4;             // waves per workgroup
+constexpr int GR_PAD = 32;              // rows behind the last one that may be read (and are not used)
 constexpr int GR_MAX_WAVES = 4096;      // stretches per pass: 16 waves per CU
 
 struct GrPass {                         // one lookup's copy of the rows
@@ -33,9 +34,38 @@ struct GrPass {                         // one lookup's copy of the rows
   int own, lookups;
 };
 
-// CP chains x 64 / CP rows per wave.  FIRST: this pass also takes the sums that need every row once.  With 64 chains a
-// wave's rows are the same for all lanes: y, X and the group come through scalar loads, and a row costs 2 D + 3 vector
-// instructions (hence the pointers of their own: the compiler must see that nothing here writes what they point to).
+// the workgroup's dense sums: [0] e^2, [1] e, [2 + j] e x_j; eight at a time through LDS
+template <int CP, int D, bool GRAD, int DD>
+__device__ __forceinline__ void grouped_dense(double sum_sq, double sum_e, const float (&gw)[DD], int d, int C,
+                                              int chain0, double* __restrict__ dense) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cl = lane % CP, q = lane / CP;
+  constexpr int COUNT = GRAD ? 2 + D : 1;
+  const int count = GRAD ? 2 + d : 1;
+  __shared__ double red[GR_WAVES][8][CP];
+#pragma unroll
+  for (int k0 = 0; k0 < COUNT; k0 += 8) {
+    __syncthreads();
+#pragma unroll
+    for (int k = k0; k < k0 + 8 && k < COUNT; ++k) {
+      double v = k == 0 ? sum_sq : k == 1 ? sum_e : (double)gw[k >= 2 ? k - 2 : 0];
+#pragma unroll
+      for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+      if (q == 0) red[wave][k - k0][cl] = v;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < 8 * CP; t += 64 * GR_WAVES) {
+      const int k = k0 + t / CP, ch = chain0 + t % CP;
+      if (k < count && ch < C) {
+        double v = 0.0;
+#pragma unroll
+        for (int x = 0; x < GR_WAVES; ++x) v += red[x][t / CP][t % CP];
+        dense[((int64_t)blockIdx.x * count + k) * C + ch] = v;
+      }
+    }
+  }
+}
+
+// CP chains x 64 / CP rows per wave (up to 16 chains).  FIRST: this pass also takes the sums that need every row once.
 template <int CP, int D, bool GRAD, bool FIRST>
 __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
     GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
@@ -124,31 +154,213 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
     i0 = e0;
   }
   if (!FIRST) return;
-  // the workgroup's dense sums: [0] e^2, [1] e, [2 + j] e x_j; eight at a time through LDS
-  constexpr int COUNT = GRAD ? 2 + D : 1;
-  const int count = GRAD ? 2 + d : 1;
-  __shared__ double red[GR_WAVES][8][CP];
+  grouped_dense<CP, D, GRAD>(sum_sq, sum_e, gw, d, C, blockIdx.y * CP, dense);
+}
+
+// 64 chains per wave: 32 lanes of two chains each times two rows.  A wave keeps 32 rows in LDS (its own part: no
+// barriers) and has the next ones on their way in registers, long enough to hide their latency; a row's features are then
+// read by broadcast, once for two chains.  What remains is 2 D + 3 vector instructions per row and chain.  Read straight
+// from memory through scalar loads, rows cost 81 us at 1M rows, D = 8, 64 chains; with the next block of scalars on its
+// way too many registers (93 us).  OTHERS: tables beside the own one (2: any number beyond one).
+// Beyond 16 features a lane has registers for one chain, and the tile is 16 rows.
+template <int D, bool GRAD, bool FIRST, int OTHERS>
+__global__ __launch_bounds__(64 * GR_WAVES) void grouped_wide_kernel(
+    GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
+    const float* __restrict__ zown, const int32_t* __restrict__ start, int64_t n, int d, int64_t span, int C, int64_t P,
+    const float* __restrict__ theta, const float* __restrict__ tables, float* __restrict__ slots,
+    double* __restrict__ dense) {
+  constexpr int K = D <= 16 ? 2 : 1, CL = 64 / K, DD = D ? D : 1;
+  constexpr int GR_TILE = D <= 16 ? 32 : 16;
+  constexpr int XV = D ? (GR_TILE * D + 255) / 256 : 1;           // 16-byte loads per lane and tile
+  constexpr int IDS = OTHERS ? BVI_MAX_LOOKUPS : 1;
+  __shared__ f32x4 lds_x[GR_WAVES][D ? GR_TILE * D / 4 + 1 : 1];
+  __shared__ float lds_y[GR_WAVES][GR_TILE], lds_z[GR_WAVES][GR_TILE];
+  __shared__ int lds_id[GR_WAVES][IDS][GR_TILE];
+  const int lane = threadIdx.x & 63, cl = lane % CL, q = lane / CL;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int c[K];
+  bool live[K];
+  float b[K], w[K][DD], gw[K][DD];
+  double sum_e[K] = {}, sum_sq[K] = {};
 #pragma unroll
-  for (int k0 = 0; k0 < COUNT; k0 += 8) {
-    __syncthreads();
+  for (int k = 0; k < K; ++k) {
+    const int chain = blockIdx.y * 64 + k * CL + cl;
+    live[k] = chain < C;
+    c[k] = live[k] ? chain : C - 1;
+    const float* th = theta + (int64_t)c[k] * P;
+    b[k] = th[0];
 #pragma unroll
-    for (int k = k0; k < k0 + 8 && k < COUNT; ++k) {
-      double v = k == 0 ? sum_sq : k == 1 ? sum_e : (double)gw[k >= 2 ? k - 2 : 0];
-#pragma unroll
-      for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
-      if (q == 0) red[wave][k - k0][cl] = v;
-    }
-    __syncthreads();
-    for (int t = threadIdx.x; t < 8 * CP; t += 64 * GR_WAVES) {
-      const int k = k0 + t / CP, ch = blockIdx.y * CP + t % CP;
-      if (k < count && ch < C) {
-        double v = 0.0;
-#pragma unroll
-        for (int x = 0; x < GR_WAVES; ++x) v += red[x][t / CP][t % CP];
-        dense[((int64_t)blockIdx.x * count + k) * C + ch] = v;
-      }
+    for (int j = 0; j < DD; ++j) {
+      w[k][j] = j < d ? th[1 + j] : 0.f;
+      gw[k][j] = 0.f;
     }
   }
+  const int own = a.own, rows = (int)a.rows[own];
+  const int64_t wid = (int64_t)blockIdx.x * GR_WAVES + wave;
+  const int64_t begin = wid * span, end = begin + span < n ? begin + span : n;
+  if (begin < end) {
+    // group g's end and the own table's entries, and those of group g + 1 (end -1: there is none); rows without a group
+    // come last, as one group whose number is `rows`
+    int g;
+    int64_t e0, next_end;
+    float u[K], next_u[K], se[K] = {}, sq[K] = {}, su[K] = {};
+    auto effect = [&](int v, float (&to)[K]) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        to[k] = tables ? tables[(a.at[own] + v) * C + c[k]] : theta[(int64_t)c[k] * P + a.offset[own] + v];
+    };
+    auto look_ahead = [&]() {
+      next_end = g + 1 < rows ? (int64_t)start[g + 2] : -1;
+      if (g + 1 < rows) effect(g + 1, next_u);
+    };
+    auto look_up = [&](int64_t i) {
+      g = __builtin_amdgcn_readfirstlane(key[i]);
+      const bool inside = g >= 0 && g < rows;
+      g = inside ? g : rows;
+      e0 = inside ? (int64_t)start[g + 1] : end;
+#pragma unroll
+      for (int k = 0; k < K; ++k) u[k] = 0.f;
+      if (inside) effect(g, u);
+      look_ahead();
+    };
+    // a tile's rows, one part per lane
+    f32x4 px[XV];
+    float py, pz = 1.f;
+    int pid[IDS];
+    auto fetch = [&](int64_t i) {
+      if (D > 0) {
+#pragma unroll
+        for (int v = 0; v < XV; ++v)
+          if ((v * 64 + lane) * 4 < GR_TILE * D) px[v] = *reinterpret_cast<const f32x4*>(X + i * D + (v * 64 + lane) * 4);
+      }
+      if (lane < GR_TILE) {
+        py = y[i + lane];
+        if (zown) pz = zown[i + lane];
+        if (OTHERS)
+#pragma unroll
+          for (int l = 0; l < IDS; ++l)
+            if (l < a.lookups) pid[l] = a.id[l][i + lane];
+      }
+    };
+    auto keep = [&]() {
+      __builtin_amdgcn_wave_barrier();
+      if (D > 0) {
+#pragma unroll
+        for (int v = 0; v < XV; ++v)
+          if ((v * 64 + lane) * 4 < GR_TILE * D) lds_x[wave][v * 64 + lane] = px[v];
+      }
+      if (lane < GR_TILE) {
+        lds_y[wave][lane] = py;
+        lds_z[wave][lane] = pz;
+        if (OTHERS)
+#pragma unroll
+          for (int l = 0; l < IDS; ++l)
+            if (l < a.lookups) lds_id[wave][l][lane] = pid[l];
+      }
+      __builtin_amdgcn_wave_barrier();
+    };
+    auto close = [&]() {                              // the running sums of group g end here
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (FIRST) {
+          sum_sq[k] += (double)sq[k];
+          sum_e[k] += (double)se[k];
+          sq[k] = 0.f;
+        }
+        if (GRAD) {
+          float v = zown ? su[k] : se[k];
+          if (K == 2) v += __shfl_xor(v, 32, 64);
+          if (g < rows && live[k] && q == 0) slots[(g + wid) * C + c[k]] = v;
+          se[k] = su[k] = 0.f;
+        }
+      }
+    };
+    const float* tx = reinterpret_cast<const float*>(lds_x[wave]);
+    fetch(begin);
+    look_up(begin);
+    for (int64_t i0 = begin; i0 < end; i0 += GR_TILE) {
+      keep();
+      if (i0 + GR_TILE < end) fetch(i0 + GR_TILE);
+      const int count = (int)(end - i0 < GR_TILE ? end - i0 : GR_TILE);
+      int p = 0;
+      while (true) {
+        const int64_t left = e0 - i0;
+        const int to = left < count ? (int)left : count;
+#pragma unroll 2
+        for (; p < to; p += K) {
+          const bool in = p + q < to;
+          const int r = in ? p + q : p;
+          const float yr = lds_y[wave][r];
+          const float zr = zown ? lds_z[wave][r] : 1.f;
+          float x[DD];
+          if (D >= 4) {
+#pragma unroll
+            for (int j = 0; j < D; j += 4) {
+              const f32x4 t = lds_x[wave][(r * D + j) / 4];
+#pragma unroll
+              for (int m = 0; m < 4; ++m) x[j + m < DD ? j + m : 0] = t[m];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < D; ++j) x[j] = tx[r * D + j];
+          }
+          float e[K];
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            e[k] = yr - b[k];
+            e[k] = zown ? fmaf(-u[k], zr, e[k]) : e[k] - u[k];
+          }
+          if (OTHERS) {
+#pragma unroll
+            for (int l = 0; l < (OTHERS == 1 ? 2 : IDS); ++l) {
+              if (l == own || l >= a.lookups) continue;
+              const int m = lds_id[wave][l][r];
+              const bool has = m >= 0 && m < (int)a.rows[l];
+              const float zl = a.z[l] ? a.z[l][i0 + r] : 1.f;
+#pragma unroll
+              for (int k = 0; k < K; ++k) {
+                const float t = tables[(a.at[l] + (has ? m : 0)) * C + c[k]];
+                e[k] = has ? fmaf(-t, zl, e[k]) : e[k];
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int j = 0; j < D; ++j) e[k] = fmaf(-w[k][j], x[j], e[k]);
+            e[k] = in ? e[k] : 0.f;
+            if (FIRST) sq[k] = fmaf(e[k], e[k], sq[k]);
+            if (GRAD) se[k] += e[k];
+            if (GRAD && zown) su[k] = fmaf(e[k], zr, su[k]);
+            if (FIRST && GRAD) {
+#pragma unroll
+              for (int j = 0; j < D; ++j) gw[k][j] = fmaf(e[k], x[j], gw[k][j]);
+            }
+          }
+        }
+        p = to;
+        if (p == count) break;
+        close();
+        if (next_end > e0) {                          // group g + 1 has rows, as most have
+          ++g;
+          e0 = next_end;
+#pragma unroll
+          for (int k = 0; k < K; ++k) u[k] = next_u[k];
+          look_ahead();
+        } else {
+          look_up(i0 + p);
+        }
+      }
+      if (e0 == i0 + count && e0 < end) {             // a group that ends with the tile
+        close();
+        look_up(e0);
+      }
+    }
+    close();
+  }
+  if (FIRST)
+#pragma unroll
+    for (int k = 0; k < K; ++k) grouped_dense<CL, D, GRAD>(sum_sq[k], sum_e[k], gw[k], d, C, blockIdx.y * 64 + k * CL, dense);
 }
 
 // theta's tables [C, rows] -> [rows, C], 64 x 64 through LDS
@@ -333,12 +545,12 @@ Layout layout(int64_t n, int d, int lookups, int64_t rows, unsigned columns) {
   Layout t;
   int64_t at = 0;
   t.start = at; at += words(rows + 1);
-  t.y = at; at += words(n);
-  t.X = at; at += words(n * padded_d(d));
+  t.y = at; at += words(n + GR_PAD);
+  t.X = at; at += words((n + GR_PAD) * padded_d(d));
   for (int l = 0; l < lookups; ++l) {
-    t.id[l] = at; at += words(n);
+    t.id[l] = at; at += words(n + GR_PAD);
     t.z[l] = -1;
-    if (columns >> l & 1u) { t.z[l] = at; at += words(n); }
+    if (columns >> l & 1u) { t.z[l] = at; at += words(n + GR_PAD); }
   }
   t.all = at;
   return t;
@@ -354,7 +566,7 @@ int chain_lanes(int C) { return bvi_chain_pack(C); }
 int64_t span_of(int64_t n, int C) {
   const int64_t least = 2 * (64 / chain_lanes(C)) > 16 ? 2 * (64 / chain_lanes(C)) : 16;
   const int64_t even = (n + GR_MAX_WAVES - 1) / GR_MAX_WAVES;
-  return even > least ? even : least;
+  return ((even > least ? even : least) + 3) / 4 * 4;        // a stretch starts on a 16-byte boundary
 }
 int64_t waves_of(int64_t n, int C) { const int64_t s = span_of(n, C); return n > 0 ? (n + s - 1) / s : 1; }
 int64_t blocks_of(int64_t n, int C) { return (waves_of(n, C) + GR_WAVES - 1) / GR_WAVES; }
@@ -381,6 +593,17 @@ Space space(int64_t n, int d, int lookups, const int64_t* rows, int C) {
 template <int CP, int D, bool GRAD, bool FIRST>
 void launch_pass(const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P, const float* theta,
                  const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
+  if constexpr (CP == 64) {
+    const dim3 grid(blocks, bvi_ceil_div(C, CP));
+#define GR_WIDE(N)                                                                                                     \
+  hipLaunchKernelGGL((grouped_wide_kernel<D, GRAD, FIRST, N>), grid, dim3(64 * GR_WAVES), 0, s, a, a.y, a.X, a.id[a.own], \
+                     a.z[a.own], a.start, n, d, span, C, P, theta, tables, slots, dense)
+    if (a.lookups == 1) GR_WIDE(0);
+    else if (a.lookups == 2) GR_WIDE(1);
+    else GR_WIDE(2);
+#undef GR_WIDE
+    return;
+  }
   hipLaunchKernelGGL((grouped_kernel<CP, D, GRAD, FIRST>), dim3(blocks, bvi_ceil_div(C, CP)), dim3(64 * GR_WAVES), 0, s, a,
                      a.y, a.X, a.id[a.own], a.z[a.own], a.start, n, d, span, C, P, theta, tables, slots, dense);
 }
@@ -473,7 +696,7 @@ int bvi_grouped_ws_bytes(int64_t n, int d, int n_lookups, const int64_t* rows, i
 int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, const int64_t* rows, unsigned columns,
                           const float* theta, int n_chains, float* logp, float* grad, const double* logp_ref, void* ws,
                           size_t ws_bytes, void* stream) {
-  if (!packed || !shape_ok(n, d, n_lookups, rows) || !theta || n_chains < 1 || !logp) return BVI_ERR_ARG;
+  if (!packed || (uintptr_t)packed % 16 || !shape_ok(n, d, n_lookups, rows) || !theta || n_chains < 1 || !logp) return BVI_ERR_ARG;
   if (!shape_supported(n, d, n_lookups, rows)) return BVI_ERR_UNSUPPORTED;
   if (n_chains > BVI_GROUPED_MAX_CHAINS) return BVI_ERR_UNSUPPORTED;
   const int C = n_chains;
