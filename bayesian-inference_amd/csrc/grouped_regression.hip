@@ -562,14 +562,15 @@ int64_t packed_words(int64_t n, int d, int lookups, const int64_t* rows, unsigne
 }
 
 int chain_lanes(int C) { return bvi_chain_pack(C); }
-// rows per wave: at least two per row lane, and as many as leave GR_MAX_WAVES waves busy
-int64_t span_of(int64_t n, int C) {
-  const int64_t least = 2 * (64 / chain_lanes(C)) > 16 ? 2 * (64 / chain_lanes(C)) : 16;
+// rows per wave: 16, or as many as leave GR_MAX_WAVES waves busy (not more while there are waves to spare, even where a
+// wave has 64 lanes for rows: with groups of two rows their sums follow one another, 10761 rows of one chain in 5310
+// groups took 53 us with 128 rows per wave)
+int64_t span_of(int64_t n) {
   const int64_t even = (n + GR_MAX_WAVES - 1) / GR_MAX_WAVES;
-  return ((even > least ? even : least) + 3) / 4 * 4;        // a stretch starts on a 16-byte boundary
+  return ((even > 16 ? even : 16) + 3) / 4 * 4;              // a stretch starts on a 16-byte boundary
 }
-int64_t waves_of(int64_t n, int C) { const int64_t s = span_of(n, C); return n > 0 ? (n + s - 1) / s : 1; }
-int64_t blocks_of(int64_t n, int C) { return (waves_of(n, C) + GR_WAVES - 1) / GR_WAVES; }
+int64_t waves_of(int64_t n) { const int64_t s = span_of(n); return n > 0 ? (n + s - 1) / s : 1; }
+int64_t blocks_of(int64_t n) { return (waves_of(n) + GR_WAVES - 1) / GR_WAVES; }
 
 // 4-byte words of the workspace: the dense sums, the transposed tables, the slots of every lookup
 struct Space {
@@ -578,13 +579,13 @@ struct Space {
 Space space(int64_t n, int d, int lookups, const int64_t* rows, int C) {
   Space t;
   int64_t at = 0;
-  t.dense = at; at += words(2 * blocks_of(n, C) * (2 + d) * C);
+  t.dense = at; at += words(2 * blocks_of(n) * (2 + d) * C);
   int64_t sum = 0;
   for (int l = 0; l < lookups; ++l) sum += rows[l];
   t.tables = at; at += lookups > 1 ? words(sum * C) : 0;
   for (int l = 0; l < lookups; ++l) {
     t.slots[l] = at;
-    at += words((rows[l] + GR_WAVES * blocks_of(n, C)) * C);
+    at += words((rows[l] + GR_WAVES * blocks_of(n)) * C);
   }
   t.all = at;
   return t;
@@ -703,8 +704,8 @@ int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, c
   const Space t = space(n, d, n_lookups, rows, C);
   if (!ws || ws_bytes < 4 * (size_t)t.all) return BVI_ERR_WORKSPACE;
   const hipStream_t s = (hipStream_t)stream;
-  const int64_t span = span_of(n, C);
-  const int blocks = (int)blocks_of(n, C), cp = chain_lanes(C), count = grad ? 2 + d : 1;
+  const int64_t span = span_of(n);
+  const int blocks = (int)blocks_of(n), cp = chain_lanes(C), count = grad ? 2 + d : 1;
   int64_t P = d + 2, sum = 0;
   for (int l = 0; l < n_lookups; ++l) P += rows[l];
   float* w = (float*)ws;

@@ -333,7 +333,8 @@ __global__ __launch_bounds__(256) void sort_start_kernel(const uint32_t* __restr
 //   the registers of a wave that hides as much: 65537 x 640 bf16 into 100003 rows 66 us with four, 41 with two, which is
 //   5.2 TB/s);
 //   narrow rows: a wave per row, LE lanes across the columns times Q = 64 / LE over the positions (2M x 16 into 5000 rows
-//   14 us after 29 us for the blocks of 128; a thread per vector took 43 after 42).
+//   14 us after 29 us for the blocks of 128; a thread per vector took 43 after 42; waves that walk the sorted positions and
+//   read everything once 41 - 51, since a gathered row of 64 bytes costs the 128 of its line whoever reads it).
 constexpr int GRAD_LEVELS = 8;
 struct GradLevels {
   int count, chunk_bits, fan_bits;
@@ -693,13 +694,14 @@ GradLevels grad_levels(int64_t n, int64_t width, bool wave) {
   t.count = 0;
   t.n[0] = 0;
   t.chunk_bits = wave ? 7 : 4;
-  t.fan_bits = wave ? 6 : 4;
+  t.fan_bits = wave ? 6 : 5;
   int64_t at = 0, m = n >> t.chunk_bits;
   while (t.count < GRAD_LEVELS && m >= 4) {
     t.n[t.count] = m;
     t.at[t.count] = at;
     at += level_space(m * width);
     ++t.count;
+    if (m <= 128) break;                          // a launch costs as much as the longest row's 128 vectors
     m >>= t.fan_bits;
   }
   return t;
