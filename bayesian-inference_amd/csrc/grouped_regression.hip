@@ -65,16 +65,20 @@ __device__ __forceinline__ void grouped_dense(double sum_sq, double sum_e, const
   }
 }
 
-// CP chains x 64 / CP rows per wave (up to 16 chains).  FIRST: this pass also takes the sums that need every row once.
+// Up to 16 chains: CP chains x Q = 64 / CP rows per wave, every lane its own row with its own group's effect, so that
+// groups of a few rows keep all lanes busy.  Rows are sorted by group: Q rows of one group are added lane by lane; where
+// they are of several, log2 Q shuffles leave each one's sum in its first lane (300k rows of one chain in 100k groups 10 us
+// of 5 MB; a wave that took the groups one by one 32).  FIRST: this pass also takes the sums that need
+// every row once.
 template <int CP, int D, bool GRAD, bool FIRST>
 __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
     GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
-    const float* __restrict__ zown, const int32_t* __restrict__ start, int64_t n, int d, int64_t span, int C, int64_t P,
-    const float* __restrict__ theta, const float* __restrict__ tables, float* __restrict__ slots,
-    double* __restrict__ dense) {
+    const float* __restrict__ zown, int64_t n, int d, int64_t span, int C, int64_t P, const float* __restrict__ theta,
+    const float* __restrict__ tables, float* __restrict__ slots, double* __restrict__ dense) {
   constexpr int Q = 64 / CP;
   constexpr int DD = D ? D : 1;
-  constexpr int U = D <= 16 ? 4 : 1;                       // rows in flight
+  constexpr int U = D <= 16 ? 4 : 1;                       // rows per lane in flight
+  constexpr int NONE = -2147483647 - 1;
   const int lane = threadIdx.x & 63, cl = lane % CP, q = lane / CP;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chain = blockIdx.y * CP + cl;
@@ -89,72 +93,118 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
     gw[j] = 0.f;
   }
   double sum_e = 0.0, sum_sq = 0.0;
-  const int own = a.own;
-  const int64_t rows = a.rows[own];
+  const int own = a.own, rows = (int)a.rows[own];
   const int64_t wid = (int64_t)blockIdx.x * GR_WAVES + wave;
-  int64_t i0 = wid * span;
-  const int64_t end = i0 + span < n ? i0 + span : n;
-  while (i0 < end) {
-    const int g = __builtin_amdgcn_readfirstlane(key[i0]);
-    const bool inside = g >= 0 && g < rows;
-    int64_t e0 = inside ? (int64_t)__builtin_amdgcn_readfirstlane(start[g + 1]) : end;
-    if (e0 > end) e0 = end;
-    const float u = !inside ? 0.f : tables ? tables[(a.at[own] + g) * C + c] : th[a.offset[own] + g];
-    const float base = zown ? b : b + u;
-    float se = 0.f, sq = 0.f, su = 0.f;
-    auto row = [&](float yi, const float* x, float zo, int64_t i) {
-      float r = yi - base;
-      if (zown) r = fmaf(-u, zo, r);
+  const int64_t begin = wid * span, end = begin + span < n ? begin + span : n;
+  int run_key = NONE;                                      // the group whose sum is not over yet, and every lane's part
+  float run = 0.f;
+  int kept_key = NONE;
+  float kept = 0.f;
+  auto total = [&](float v) {
+#pragma unroll
+    for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+    return v;
+  };
+  auto put = [&](int g, float v) {
+    if (g >= 0 && g < rows && live) slots[(g + wid) * C + c] = v;
+  };
+  for (int64_t i0 = begin; i0 < end; i0 += U * Q) {
+    float e[U], zo[U], u[U];
+    int k[U];
+    float se = 0.f, sq = 0.f;
+    auto at = [&](int t) { return i0 + t * Q + q < end ? i0 + t * Q + q : end - 1; };
+    auto effect = [&](int g) {
+      if (g < 0 || g >= rows) g = 0;                       // not used
+      return tables ? tables[(a.at[own] + g) * C + c] : th[a.offset[own] + g];
+    };
+    float x[U][DD], yt[U];                                 // every row's loads leave before the first is waited for
+#pragma unroll
+    for (int t = 0; t < U; ++t) {
+      const int64_t i = at(t);
+      k[t] = key[i];
+      yt[t] = y[i];
+      zo[t] = zown ? zown[i] : 1.f;
+#pragma unroll
+      for (int j = 0; j < D; ++j) x[t][j] = X[i * D + j];
+    }
+    // one entry per chain while a group lasts: a gather for every row touches a line per lane
+    if (__builtin_amdgcn_readfirstlane(k[0]) == __builtin_amdgcn_readlane(k[U - 1], 63)) {
+      if (k[0] != kept_key) kept = effect(k[0]);
+      kept_key = k[0];
+#pragma unroll
+      for (int t = 0; t < U; ++t) u[t] = kept;
+    } else {
+#pragma unroll
+      for (int t = 0; t < U; ++t) u[t] = effect(k[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < U; ++t) {
+      const bool in = i0 + t * Q + q < end;
+      const int64_t i = at(t);
+      float r = yt[t] - b;
+      r = k[t] >= 0 && k[t] < rows ? fmaf(-u[t], zo[t], r) : r;
       for (int l = 0; l < a.lookups; ++l) {
         if (l == own) continue;
-        const int64_t k = a.id[l][i];
-        if (k >= 0 && k < a.rows[l]) r -= tables[(a.at[l] + k) * C + c] * (a.z[l] ? a.z[l][i] : 1.f);
+        const int64_t m = a.id[l][i];
+        if (m >= 0 && m < a.rows[l]) r -= tables[(a.at[l] + m) * C + c] * (a.z[l] ? a.z[l][i] : 1.f);
       }
-      if (D > 0) {
 #pragma unroll
-        for (int j = 0; j < D; ++j) r = fmaf(-w[j], x[j], r);
-      }
+      for (int j = 0; j < D; ++j) r = fmaf(-w[j], x[t][j], r);
+      r = in ? r : 0.f;
+      k[t] = in ? k[t] : NONE;
+      e[t] = r;
       if (FIRST) sq = fmaf(r, r, sq);
-      if (GRAD) se += r;
-      if (GRAD && zown) su = fmaf(r, zo, su);
-      if (FIRST && GRAD && D > 0) {
+      if (FIRST && GRAD) {
+        se += r;
 #pragma unroll
-        for (int j = 0; j < D; ++j) gw[j] = fmaf(r, x[j], gw[j]);
+        for (int j = 0; j < D; ++j) gw[j] = fmaf(r, x[t][j], gw[j]);
       }
-    };
-    int64_t i = i0 + q;
-    for (; i + (U - 1) * Q < e0; i += U * Q) {
-      float yi[U], zo[U], x[U][DD];
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        yi[k] = y[i + k * Q];
-        zo[k] = zown ? zown[i + k * Q] : 1.f;
-#pragma unroll
-        for (int j = 0; j < D; ++j) x[k][j] = X[(i + k * Q) * D + j];
-      }
-#pragma unroll
-      for (int k = 0; k < U; ++k) row(yi[k], x[k], zo[k], i + k * Q);
-    }
-    for (; i < e0; i += Q) {
-      float x[DD];
-#pragma unroll
-      for (int j = 0; j < D; ++j) x[j] = X[i * D + j];
-      row(y[i], x, zown ? zown[i] : 1.f, i);
     }
     if (FIRST) {
       sum_sq += (double)sq;
       sum_e += (double)se;
     }
-    if (GRAD && inside) {
-      float v = zown ? su : se;
+    if (GRAD) {
 #pragma unroll
-      for (int off = CP; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
-      if (q == 0 && live) slots[(g + wid) * C + c] = v;
+      for (int t = 0; t < U; ++t) {
+        float v = e[t] * zo[t];
+        const int first = __builtin_amdgcn_readfirstlane(k[t]), last = __builtin_amdgcn_readlane(k[t], 63);
+        if (first == last) {                               // all of one group: no shuffles while it lasts
+          if (first == run_key) {
+            run += v;
+          } else {
+            run = total(run);
+            if (q == 0) put(run_key, run);
+            run_key = first;
+            run = v;
+          }
+          continue;
+        }
+        const float carry = total(run);
+#pragma unroll
+        for (int off = 1; off < Q; off <<= 1) {            // the sum from here to the group's end within these rows
+          const float more = __shfl_down(v, off * CP, 64);
+          const int there = __shfl_down(k[t], off * CP, 64);
+          v += q + off < Q && there == k[t] ? more : 0.f;
+        }
+        const int left = __shfl_up(k[t], CP, 64);
+        const bool head = q == 0 || left != k[t];
+        if (q == 0) {
+          if (first == run_key) v += carry;
+          else put(run_key, carry);
+        }
+        if (head && k[t] != last) put(k[t], v);
+        // the last group goes on: its first lane here keeps its sum
+        run = head && k[t] == last ? v : 0.f;
+        run_key = last;
+      }
     }
-    i0 = e0;
   }
-  if (!FIRST) return;
-  grouped_dense<CP, D, GRAD>(sum_sq, sum_e, gw, d, C, blockIdx.y * CP, dense);
+  if (GRAD) {
+    run = total(run);
+    if (q == 0) put(run_key, run);
+  }
+  if (FIRST) grouped_dense<CP, D, GRAD>(sum_sq, sum_e, gw, d, C, blockIdx.y * CP, dense);
 }
 
 // 64 chains per wave: 32 lanes of two chains each times two rows.  A wave keeps 32 rows in LDS (its own part: no
@@ -562,9 +612,7 @@ int64_t packed_words(int64_t n, int d, int lookups, const int64_t* rows, unsigne
 }
 
 int chain_lanes(int C) { return bvi_chain_pack(C); }
-// rows per wave: 16, or as many as leave GR_MAX_WAVES waves busy (not more while there are waves to spare, even where a
-// wave has 64 lanes for rows: with groups of two rows their sums follow one another, 10761 rows of one chain in 5310
-// groups took 53 us with 128 rows per wave)
+// rows per wave: 16, or as many as leave GR_MAX_WAVES waves busy
 int64_t span_of(int64_t n) {
   const int64_t even = (n + GR_MAX_WAVES - 1) / GR_MAX_WAVES;
   return ((even > 16 ? even : 16) + 3) / 4 * 4;              // a stretch starts on a 16-byte boundary
@@ -606,7 +654,7 @@ void launch_pass(const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t
     return;
   }
   hipLaunchKernelGGL((grouped_kernel<CP, D, GRAD, FIRST>), dim3(blocks, bvi_ceil_div(C, CP)), dim3(64 * GR_WAVES), 0, s, a,
-                     a.y, a.X, a.id[a.own], a.z[a.own], a.start, n, d, span, C, P, theta, tables, slots, dense);
+                     a.y, a.X, a.id[a.own], a.z[a.own], n, d, span, C, P, theta, tables, slots, dense);
 }
 template <int CP, int D>
 void launch_pass_mode(bool grad, bool first, const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P,
