@@ -71,8 +71,7 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, plan=None):
     g, stride = _rows_view(grad_out.reshape(n, width), 'grad_out')
     if plan is not None:
         plan.check(n, num_rows, g.device)
-    else:
-        ids = ids.contiguous()
+    ids = ids.contiguous()
     out = torch.empty((num_rows,) if flat else (num_rows, width), dtype=g.dtype, device=g.device)
     _native.lookup_grad(g, n, width, stride, ids, None if plan is None else plan.buffer, num_rows, float(scale), out)
     return out

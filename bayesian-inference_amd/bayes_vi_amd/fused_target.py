@@ -213,7 +213,10 @@ class GroupedRegression(FusedLogLikelihood):
         columns = [None] * len(self.rows) if columns is None else list(columns)
         if not 1 <= len(self.rows) <= _native.MAX_LOOKUPS or len(ids) != len(self.rows) or len(columns) != len(self.rows):
             raise ValueError('one id column (and one entry of `columns`) for each of 1 to %d tables' % _native.MAX_LOOKUPS)
-        X = None if X is None else X.to(torch.float32).reshape(self.n, -1).contiguous() if self.n else X.to(torch.float32)
+        if X is not None:
+            X = (X[:, None] if X.dim() == 1 else X).to(torch.float32).contiguous()
+            if X.dim() != 2 or X.shape[0] != self.n or X.device != self.y.device:
+                raise ValueError('X must be [%d, D] on %s, got %s on %s' % (self.n, self.y.device, tuple(X.shape), X.device))
         self.d = 0 if X is None else X.shape[1]
         if self.d > 64:
             raise ValueError('at most 64 feature columns beside the group effects, got %d' % self.d)
@@ -234,8 +237,12 @@ class GroupedRegression(FusedLogLikelihood):
         self._sizes = _native._int64s(self.rows)
 
     def _call(self, theta, logp, grad, relative=False):
+        _native._check_f32_cuda(theta)
+        if theta.dim() != 2 or theta.shape[1] != self.n_params:
+            raise ValueError('theta must be [chains, %d], got %s' % (self.n_params, tuple(theta.shape)))
         c = theta.shape[0]
-        buf = self.ws.get(_native.grouped_ws_bytes(self.n, self.d, self.rows, c))
+        # scratch of this call: a captured graph keeps its own, whatever later calls need
+        buf = _native._scratch(_native.grouped_ws_bytes(self.n, self.d, self.rows, c), self.device)
         _launch(_native.lib().bvi_grouped_logp_grad, _native._ptr(self.packed), self.n, self.d, len(self.rows), self._sizes,
                 self.mask, _native._ptr(theta), c, _native._ptr(logp), _native._ptr(grad), self._ref(relative),
                 _native._ptr(buf), buf.numel(), _native._stream())

@@ -83,6 +83,8 @@ class _AdamState:
             self.step()
             return
         if self.global_clipnorm is not None or any(p.numel() > ONE_WORKGROUP_MAX for p, _, _, _ in live):
+            if len({id(p) for p, _, _, _ in live}) != len(live):
+                raise ValueError('a variable is in the optimiser twice: the step over the list would write it twice at once')
             hyper = (self.lr, self.b1, self.b2, self.eps)
             if self.global_clipnorm is None:      # the constants that bvi_clip_adam_step takes: same results to rounding
                 hyper = tuple(float(np.float32(h)) for h in hyper)

@@ -82,6 +82,7 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
             out = [torch.empty_like(t) for t in src]
     norm = _native.clip_by_global_norm(src, out, clip_norm, use_norm, device)
     if inplace:
+        torch.autograd.graph.increment_version(live)
         return list(t_list), norm
     if len(live) == len(t_list):
         return out, norm

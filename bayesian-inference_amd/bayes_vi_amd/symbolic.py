@@ -177,9 +177,9 @@ def gather(params, indices):
     import torch
     if isinstance(params, torch.Tensor) and isinstance(indices, torch.Tensor):
         ids = whole_numbers(indices.reshape(-1))
+        if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= params.shape[-1]):
+            raise IndexError('gather: an index lies outside [0, %d)' % params.shape[-1])
         if not params.is_cuda:                      # draws of a prior live on the host
-            if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= params.shape[-1]):
-                raise IndexError('gather: an index lies outside [0, %d)' % params.shape[-1])
             return params[..., ids.to(params.device)]
         from . import embedding
         table = params.reshape(-1, params.shape[-1]).T

@@ -582,9 +582,12 @@ bool shape_ok(int64_t n, int d, int lookups, const int64_t* rows) {
 }
 bool shape_supported(int64_t n, int d, int lookups, const int64_t* rows) {
   if (d > 64 || lookups > BVI_MAX_LOOKUPS || n > BVI_LOOKUP_MAX) return false;
-  for (int l = 0; l < lookups; ++l)
-    if (rows[l] > (1 << 25)) return false;               // threads of the finishing launch: 64 per row
-  return true;
+  int64_t all = 0;
+  for (int l = 0; l < lookups; ++l) {
+    if (rows[l] > (1 << 25)) return false;
+    all += rows[l];
+  }
+  return all <= (1 << 25);                          // the finishing launch has up to 64 threads for each
 }
 
 // 4-byte words of one copy: start, y, X, and per lookup the groups and, where there is one, the column
@@ -706,6 +709,7 @@ int bvi_grouped_pack(const float* X, const float* y, int64_t n, int d, int n_loo
   size_t need, scratch;
   bvi_grouped_packed_bytes(n, d, n_lookups, rows, mask, &need, &scratch);
   if (!packed || packed_bytes < need || !ws || ws_bytes < scratch) return BVI_ERR_WORKSPACE;
+  if (((uintptr_t)packed | (uintptr_t)ws) % 16) return BVI_ERR_ARG;
   const hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)((n + 255) / 256));
   float* base = (float*)packed;
@@ -751,6 +755,7 @@ int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, c
   const int C = n_chains;
   const Space t = space(n, d, n_lookups, rows, C);
   if (!ws || ws_bytes < 4 * (size_t)t.all) return BVI_ERR_WORKSPACE;
+  if ((uintptr_t)ws % 16) return BVI_ERR_ARG;
   const hipStream_t s = (hipStream_t)stream;
   const int64_t span = span_of(n);
   const int blocks = (int)blocks_of(n), cp = chain_lanes(C), count = grad ? 2 + d : 1;

@@ -422,16 +422,18 @@ __global__ __launch_bounds__(256) void grad_level_kernel(const S* __restrict__ s
   const int per = LE ? 4 : 256 / tc, sub = LE ? threadIdx.x >> 6 : threadIdx.x / tc;
   const int t = LE ? threadIdx.x & 63 : threadIdx.x - sub * tc, step = LE ? LE : tc;
   const int q = LE ? t / step : 0, col0 = LE ? t % step : t;
-  const int64_t b = (int64_t)blockIdx.x * per + sub;
-  if (sub >= per || b >= n_blocks) return;
-  const uint32_t k0 = key[b << span_bits];
-  if (k0 != key[((b + 1) << span_bits) - 1] || k0 >= rows) return;
-  for (int col = col0; col - col0 < W; col += step) {
-    float acc[V] = {};
-    if (col < W)
-      grad_sum<S, V, PERM, Q, LE ? 8 : 4>(acc, src, stride, (int64_t)col * V, order, (int)(b << bits) + q, (int)((b + 1) << bits));
-    if (LE) grad_join<V, LE ? LE : 64>(acc);
-    if (q == 0 && col < W) grad_store<float, V>(sums + (b * W + col) * V, acc);
+  if (sub >= per) return;
+  for (int64_t b = (int64_t)blockIdx.x * per + sub; b < n_blocks; b += (int64_t)gridDim.x * per) {
+    const uint32_t k0 = key[b << span_bits];
+    if (k0 != key[((b + 1) << span_bits) - 1] || k0 >= rows) continue;
+    for (int col = col0; col - col0 < W; col += step) {
+      float acc[V] = {};
+      if (col < W)
+        grad_sum<S, V, PERM, Q, LE ? 8 : 4>(acc, src, stride, (int64_t)col * V, order, (int)(b << bits) + q,
+                                            (int)((b + 1) << bits));
+      if (LE) grad_join<V, LE ? LE : 64>(acc);
+      if (q == 0 && col < W) grad_store<float, V>(sums + (b * W + col) * V, acc);
+    }
   }
 }
 
@@ -711,7 +713,7 @@ int64_t level_words(int64_t n, int64_t width, bool wave) {
   return t.count ? t.at[t.count - 1] + level_space(t.n[t.count - 1] * width) : 0;
 }
 // whether looking through all ids for every row is the quickest way
-bool grad_by_scan(int64_t rows, int64_t n) { return n <= SCAN_MAX && rows * n <= (1 << 22); }
+bool grad_by_scan(int64_t rows, int64_t n) { return n <= SCAN_MAX && rows * (n > 0 ? n : 1) <= (1 << 22); }
 
 struct GradCall {
   const void* g;
@@ -738,7 +740,8 @@ int launch_grad(const GradCall& c) {
   int span_bits = 0;
   for (int l = 0; l < lv.count; ++l) {
     const int bits = l == 0 ? lv.chunk_bits : lv.fan_bits;
-    const unsigned blocks = (unsigned)((lv.n[l] + per - 1) / per);
+    const int64_t wanted = (lv.n[l] + per - 1) / per;
+    const unsigned blocks = (unsigned)(wanted < (1 << 23) ? wanted : (1 << 23));
     span_bits += bits;
     if (l == 0)
       hipLaunchKernelGGL((grad_level_kernel<T, V, LE, true>), dim3(blocks), dim3(256), 0, c.s, (const T*)c.g, c.stride, W,
@@ -805,6 +808,10 @@ int launch_grad_v(const GradCall& c) {
 #undef BVI_GRAD_CALL
 }
 
+// addresses between two elements, and scratch that the kernels' 16-byte accesses would straddle, are refused
+bool off_type(const void* p, int size) { return (uintptr_t)p % (size_t)size != 0; }
+int ids_size(int ids_type) { return ids_type == BVI_IDS_I32 ? 4 : 8; }
+
 bool sizes_ok(int64_t rows, int64_t n) {
   return rows >= 1 && rows <= BVI_LOOKUP_MAX && n >= 0 && n <= BVI_LOOKUP_MAX;
 }
@@ -819,7 +826,8 @@ int bvi_lookup(const void* table, int dtype, int64_t rows, int64_t width, int64_
   if (!table || !size || width < 1 || row_stride < width || n < 0 || rows < 1 || (n > 0 && (!ids || !out)))
     return BVI_ERR_ARG;
   if (ids_type != BVI_IDS_I32 && ids_type != BVI_IDS_I64) return BVI_ERR_ARG;
-  if (width > BVI_LOOKUP_MAX) return BVI_ERR_UNSUPPORTED;
+  if (off_type(table, size) || off_type(out, size) || off_type(ids, ids_size(ids_type))) return BVI_ERR_ARG;
+  if (width > BVI_LOOKUP_MAX || rows > BVI_LOOKUP_MAX || n > BVI_LOOKUP_MAX) return BVI_ERR_UNSUPPORTED;
   if (n == 0) return BVI_OK;
   const hipStream_t s = (hipStream_t)stream;
   const int v = vector_elements(width, row_stride, size, table, out);
@@ -843,6 +851,7 @@ int bvi_lookup_plan_bytes(int64_t rows, int64_t n, size_t* plan_bytes, size_t* w
 int bvi_lookup_plan(const void* ids, int ids_type, int64_t n, int64_t rows, void* plan, size_t plan_bytes, void* ws,
                     size_t ws_bytes, void* stream) {
   if ((!ids && n > 0) || n < 0 || rows < 1 || (ids_type != BVI_IDS_I32 && ids_type != BVI_IDS_I64)) return BVI_ERR_ARG;
+  if (off_type(ids, ids_size(ids_type)) || off_type(plan, 16) || off_type(ws, 16)) return BVI_ERR_ARG;
   if (!sizes_ok(rows, n)) return BVI_ERR_UNSUPPORTED;
   size_t need, scratch;
   bvi_lookup_plan_bytes(rows, n, &need, &scratch);
@@ -868,6 +877,9 @@ int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, i
   if ((!grad_out && n > 0) || !type_size(dtype) || n < 0 || width < 1 || row_stride < width || rows < 1 || !grad_table)
     return BVI_ERR_ARG;
   if ((!plan && !ids && n > 0) || (ids && (ids_type != BVI_IDS_I32 && ids_type != BVI_IDS_I64))) return BVI_ERR_ARG;
+  if (off_type(grad_out, type_size(dtype)) || off_type(grad_table, type_size(dtype)) ||
+      (ids && off_type(ids, ids_size(ids_type))) || off_type(plan, 16) || off_type(ws, 16))
+    return BVI_ERR_ARG;
   if (!sizes_ok(rows, n) || width > BVI_LOOKUP_MAX) return BVI_ERR_UNSUPPORTED;
   size_t need;
   bvi_lookup_grad_ws_bytes(rows, width, n, plan != nullptr, &need);

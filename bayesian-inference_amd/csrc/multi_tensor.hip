@@ -484,6 +484,7 @@ int bvi_global_norm(int n_tensors, const void* const* tensors, const int64_t* si
   size_t need;
   bvi_global_norm_ws_bytes(n_tensors, &need);
   if (!ws || ws_bytes < need) return BVI_ERR_WORKSPACE;
+  if ((uintptr_t)ws % sizeof(double)) return BVI_ERR_ARG;
   if (is_small(n_tensors, sizes)) {
     ClipArgs a;
     fill(a.in, 0, n_tensors, tensors, sizes, dtypes, MT_SMALL_ITEM);
@@ -511,6 +512,7 @@ int bvi_clip_by_global_norm(int n_tensors, const void* const* tensors, void* con
   size_t need;
   bvi_global_norm_ws_bytes(n_tensors, &need);
   if (!use_norm && (!ws || ws_bytes < need)) return BVI_ERR_WORKSPACE;
+  if ((uintptr_t)ws % sizeof(double)) return BVI_ERR_ARG;
   const hipStream_t s = (hipStream_t)stream;
   if (is_small(n_tensors, sizes)) {
     ClipArgs a;
@@ -566,7 +568,10 @@ int bvi_adam_step(int n_tensors, float* const* x, float* const* grad, float* con
                   double epsilon, float clip_norm, float global_clip_norm, void* ws, size_t ws_bytes, void* stream) {
   if (!list_ok(n_tensors, sizes) || !x || !grad || !m || !v || !step_count) return BVI_ERR_ARG;
   for (int t = 0; t < n_tensors; ++t)
-    if (sizes[t] > 0 && (!x[t] || !grad[t] || !m[t] || !v[t])) return BVI_ERR_ARG;
+    if ((sizes[t] > 0 && (!x[t] || !grad[t] || !m[t] || !v[t])) ||
+        ((uintptr_t)x[t] | (uintptr_t)grad[t] | (uintptr_t)m[t] | (uintptr_t)v[t]) % sizeof(float))
+      return BVI_ERR_ARG;
+  if ((uintptr_t)ws % sizeof(double) || (uintptr_t)step_count % sizeof(double)) return BVI_ERR_ARG;
   size_t need;
   const int st = bvi_adam_step_ws_bytes(n_tensors, sizes, &need);
   if (st) return st;

@@ -476,7 +476,8 @@ int bvi_philox_normal(uint64_t seed, uint64_t step, int n_chains, int n_params, 
  *   bvi_lookup_grad       from the ids (sorted within the call), from a plan of them (ids may be NULL), or both;
  *                         grad_table[rows, width] = scale * the sums of grad_out's rows per id, in float, rounded once;
  *                         every row is written (zeros where no id asks for it); no atomics, the same bits every time
- * dtype is that of table, out, grad_out and grad_table.  rows, width and n at most BVI_LOOKUP_MAX. */
+ * dtype is that of table, out, grad_out and grad_table.  rows, width and n at most BVI_LOOKUP_MAX.  Plans and workspaces
+ * of these and the following entry points start on a multiple of 16 bytes (else BVI_ERR_ARG). */
 #define BVI_TYPE_F32 0
 #define BVI_TYPE_BF16 1
 #define BVI_TYPE_F16 2
@@ -496,7 +497,7 @@ int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, i
 /* ---- Gaussian linear regression with group-level effects: the loss that reads such tables, with its gradient.
  *   y_i ~ Normal(b + x_i . w + sum_l z_il u_l[ids_l[i]], s);  theta = (b, w[d], s, u_1[rows_1], u_2[rows_2], ...)
  * z_l (columns[l]) may be NULL: ones.  An id outside [0, rows_l) has no effect.  d <= 64, n_lookups <=
- * BVI_MAX_LOOKUPS, rows_l <= 2^25.  `rows`, `ids` and `columns` (arrays of n_lookups) are HOST arrays; `ids[l]` and
+ * BVI_MAX_LOOKUPS, all tables together at most 2^25 rows.  `rows`, `ids` and `columns` (arrays of n_lookups) are HOST arrays; `ids[l]` and
  * `columns[l]` device pointers.  bvi_grouped_pack lays the rows out once per dataset, in every lookup's order;
  * `columns` of the other calls has bit l set where columns[l] was given.  Conventions of logp, grad, logp_ref and shards
  * as for the families above. */

@@ -136,6 +136,24 @@ def test_layouts(emb, gpu_device):
         check_lookup(emb.lookup(table, ids, scale=0.5), table, ids, 0.5)
 
 
+def test_plan_with_ids_of_another_layout(emb, gpu_device):
+    """The plan and the ids may both be used: ids that are not contiguous come in their own order."""
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(31)
+    for n in (40, 4000):
+        ids = torch.randint(0, 20, (n, 3), generator=gen, device=gpu_device).T
+        g = torch.randn(3, n, 5, generator=gen, device=gpu_device)
+        plan = emb.LookupPlan(ids, 20)
+        a = emb.lookup_grad(g, ids, 20, plan=plan)
+        check_grad(a, g, ids, 20, 1.0)
+        assert torch.equal(a, emb.lookup_grad(g, ids.contiguous(), 20))
+
+
+def test_no_positions_for_a_large_table(emb, gpu_device):
+    none = torch.zeros(0, dtype=torch.int32, device=gpu_device)
+    got = emb.lookup_grad(torch.zeros(0, 2, device=gpu_device), none, 5_000_000)
+    assert got.shape == (5_000_000, 2) and not bool(got.any())
+
+
 def test_no_ids(emb, gpu_device):
     table = torch.randn(5, 3, device=gpu_device, requires_grad=True)
     none = torch.zeros(0, dtype=torch.int64, device=gpu_device)
@@ -218,8 +236,7 @@ def test_refusals_on_the_device(emb, gpu_device):
 
 
 def test_graph_replays_follow_the_inputs(emb, gpu_device):
-    """Forward, sort and gradient recorded once and replayed on new ids and values, with eager work between; an eager
-    graph of the same leaf lives meanwhile."""
+    """Forward, sort and gradient recorded once and replayed on new ids and values, with eager work between."""
     gen = torch.Generator(device=gpu_device); gen.manual_seed(7)
     rows, width, n = 90, 20, 3000
     table = torch.randn(rows, width, generator=gen, device=gpu_device)

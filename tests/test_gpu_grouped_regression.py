@@ -156,6 +156,74 @@ def test_relative_level_and_non_finite_parameters(gpu_device):
     assert not torch.isfinite(lp3[:2]).any() and torch.equal(lp3[2], lp[2]) and torch.equal(g3[2], g[2])
 
 
+def test_graphs_keep_their_scratch(gpu_device):
+    """A captured evaluation replays correctly after the likelihood was used for more chains (more scratch) in between,
+    and two graphs of one likelihood do not share any."""
+    rng = np.random.default_rng(6)
+    X, y, ids, z, theta = make(rng, 3000, 2, [40, 6], 40)
+    lik = likelihood(X, y, ids, z, [40, 6], gpu_device)
+    th = torch.tensor(theta, device=gpu_device)
+    small = [th[:3].clone(), th[3:8].clone()]
+    want = [lik.logp_grad(t) for t in small]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for t in small:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(lik.logp_grad(t))
+    for k in range(4):
+        big = lik.logp_grad(th)
+        junk = torch.full((1 << 20,), float('nan'), device=gpu_device)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (lp, gr), (wl, wg) in zip(outs, want):
+            assert torch.equal(lp, wl) and torch.equal(gr, wg)
+        assert torch.isfinite(big[1]).all() and torch.isnan(junk).all()
+
+
+def test_theta_is_checked(gpu_device):
+    rng = np.random.default_rng(8)
+    X, y, ids, z, theta = make(rng, 50, 1, [4], 2)
+    lik = likelihood(X, y, ids, z, [4], gpu_device)
+    th = torch.tensor(theta, device=gpu_device)
+    for bad in (th[:, :-1], torch.cat([th, th], 1)):
+        with pytest.raises(ValueError, match='theta must be'):
+            lik.logp_grad(bad)
+    from bayes_vi_amd._native import BviError
+    for bad in (th.cpu(), th.double()):
+        with pytest.raises(BviError):
+            lik.logp_grad(bad)
+
+
+def test_rows_without_a_group_have_no_effect(gpu_device):
+    """The C entry point takes ids outside the table (the Python class refuses them): such rows have no effect of that
+    lookup, wherever in a stretch of rows they fall."""
+    import ctypes
+    from bayes_vi_amd import _native as nat
+    rng = np.random.default_rng(9)
+    for chains in (1, 3, 16, 40):
+        X, y, ids, z, theta = make(rng, 700, 1, [9, 5], chains)
+        for i, rows in zip(ids, (9, 5)):
+            out = rng.random(700) < 0.3
+            i[out] = rng.choice([-1, rows, rows + 3, 2 ** 31 - 1, -2 ** 31], out.sum())
+        dev = lambda a: torch.tensor(a, device=gpu_device)
+        packed, mask = nat.grouped_pack(dev(X), dev(y), [dev(i.astype(np.int32)) for i in ids], [9, 5], [None, None])
+        th = dev(theta)
+        lp, g = torch.empty(chains, device=gpu_device), torch.empty_like(th)
+        ws = nat._scratch(nat.grouped_ws_bytes(700, 1, [9, 5], chains), gpu_device)
+        nat.check(nat.lib().bvi_grouped_logp_grad(packed.data_ptr(), 700, 1, 2, nat._int64s([9, 5]), mask, th.data_ptr(), chains,
+                                                  lp.data_ptr(), g.data_ptr(), None, ws.data_ptr(), ws.numel(), nat._stream()),
+                  'bvi_grouped_logp_grad')
+        # the same with one more row in each table whose effect is zero
+        ids2 = [np.where((i >= 0) & (i < r), i, r) for i, r in zip(ids, (9, 5))]
+        th2 = np.concatenate([theta[:, :12], np.zeros((chains, 1)), theta[:, 12:], np.zeros((chains, 1))], 1).astype(np.float32)
+        rlp, rg, blp, bg = oracle(X, y, ids2, z, th2, [10, 6])
+        keep = [j for j in range(th2.shape[1]) if j not in (12, 18)]
+        assert (np.abs(lp.cpu().numpy() - rlp) <= blp).all()
+        assert (np.abs(g.cpu().numpy() - rg[:, keep]) <= bg[:, keep]).all()
+
+
 def test_refusals(gpu_device):
     from bayes_vi_amd.fused_target import GroupedRegression
     y = torch.zeros(5, device=gpu_device)
@@ -164,6 +232,8 @@ def test_refusals(gpu_device):
                 lambda: GroupedRegression(None, y, [i[:4]], [3]), lambda: GroupedRegression(None, y, [i.float()], [3]),
                 lambda: GroupedRegression(None, y, [i, i], [3]), lambda: GroupedRegression(None, y, [i] * 9, [3] * 9),
                 lambda: GroupedRegression(torch.zeros(5, 65, device=gpu_device), y, [i], [3]),
+                lambda: GroupedRegression(torch.zeros(10, device=gpu_device), y, [i], [3]),
+                lambda: GroupedRegression(torch.zeros(5, 2), y, [i], [3]),
                 lambda: GroupedRegression(None, y, [i], [3], [torch.zeros(4, device=gpu_device)])):
         with pytest.raises(ValueError):
             bad()

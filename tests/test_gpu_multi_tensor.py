@@ -192,6 +192,23 @@ def test_adam_without_a_joint_clip_keeps_its_results(gpu_device):
     assert bool(((p.detach() - x).abs() <= 2 * U * x.abs() + 0.05 * 1.1 * 32 * U).all())
 
 
+def test_a_variable_twice_is_refused(gpu_device):
+    from bayes_vi_amd.inference.vi.vi import Adam
+    p = torch.nn.Parameter(torch.ones(5, device=gpu_device))
+    p.grad = torch.ones(5, device=gpu_device)
+    with pytest.raises(ValueError, match='twice'):
+        Adam(global_clipnorm=1.0).bind([p, p]).clip_and_step(1.0)
+
+
+def test_clipping_in_place_is_seen_by_autograd(la, gpu_device):
+    x = torch.ones(4, device=gpu_device, requires_grad=True)
+    y = x * 2.0
+    z = (y * y).sum()
+    la.clip_by_global_norm([y.detach()], 0.5, inplace=True)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        z.backward()
+
+
 def test_adam_non_finite_gradient(gpu_device):
     from bayes_vi_amd.inference.vi.vi import Adam
     ps = [torch.nn.Parameter(torch.ones(5, device=gpu_device)) for _ in range(2)]

@@ -65,6 +65,13 @@ def test_c_entry_points_refuse_before_launching():
     assert lib.bvi_lookup_grad(p, 0, 5, 3, 3, p, 5, None, 4, 1.0, p, p, 16, None) == -1
     assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 0, p, 4, 1.0, p, None, 0, None) == -3
     assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 0, None, 4, 1.0, p, p, 16, None) == -3
+    # addresses between elements, scratch off its alignment
+    odd = ctypes.c_void_p(4098)
+    assert lib.bvi_lookup(odd, 0, 4, 3, 3, p, 0, 5, 1.0, p, None) == -1
+    assert lib.bvi_lookup(p, 0, 4, 3, 3, odd, 0, 5, 1.0, p, None) == -1
+    assert lib.bvi_lookup_plan(p, 1, 5000, 4, odd, 1 << 30, p, 1 << 30, None) == -1
+    assert lib.bvi_lookup_grad(p, 0, 5000, 3, 3, p, 0, None, 4, 1.0, p, odd, 1 << 30, None) == -1
+    assert lib.bvi_lookup_grad(odd, 0, 5000, 3, 3, p, 0, None, 4, 1.0, p, p, 1 << 30, None) == -1
     ptrs, types = (ctypes.c_void_p * 1)(4096), (ctypes.c_int * 1)(0)
     assert lib.bvi_global_norm(0, ptrs, one, types, p, p, 1 << 20, None) == -1
     assert lib.bvi_global_norm(1, ptrs, one, (ctypes.c_int * 1)(9), p, p, 1 << 20, None) == -1
@@ -77,7 +84,12 @@ def test_c_entry_points_refuse_before_launching():
     assert lib.bvi_grouped_packed_bytes(5, 65, 1, one, 0, ctypes.byref(z), ctypes.byref(z)) == -2
     assert lib.bvi_grouped_packed_bytes(5, 1, 9, _native._int64s([1] * 9), 0, ctypes.byref(z), ctypes.byref(z)) == -2
     assert lib.bvi_grouped_packed_bytes(5, 1, 1, _native._int64s([0]), 0, ctypes.byref(z), ctypes.byref(z)) == -1
+    assert lib.bvi_grouped_packed_bytes(5, 1, 2, _native._int64s([1 << 24, (1 << 24) + 1]), 0, ctypes.byref(z),
+                                        ctypes.byref(z)) == -2
     assert lib.bvi_grouped_ws_bytes(5, 1, 1, one, 0, ctypes.byref(z)) == -1
+    assert lib.bvi_grouped_logp_grad(odd, 5, 1, 1, one, 0, p, 4, p, p, None, p, 1 << 30, None) == -1
+    assert lib.bvi_adam_step(1, (ctypes.c_void_p * 1)(4098), ptrs, ptrs, ptrs, one, p, .1, .9, .999, 1e-7, 1., 1., p, 1 << 20,
+                             None) == -1
     assert lib.bvi_grouped_ws_bytes(5, 1, 1, one, (1 << 20) + 1, ctypes.byref(z)) == -2
     assert lib.bvi_grouped_logp_grad(p, 5, 1, 1, one, 0, p, 4, p, p, None, p, 16, None) == -3
 
