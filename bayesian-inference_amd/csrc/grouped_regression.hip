@@ -29,9 +29,13 @@ struct GrPass {                         // one lookup's copy of the rows
   const float* z[BVI_MAX_LOOKUPS];      // or NULL
   const int32_t* start;                 // of the own lookup
   int64_t rows[BVI_MAX_LOOKUPS];
-  int64_t offset[BVI_MAX_LOOKUPS];      // of u_l in theta
-  int64_t at[BVI_MAX_LOOKUPS];          // of u_l in the transposed tables
+  const float* tab[BVI_MAX_LOOKUPS];    // u_l of group g and chain c: tab[l][g group_stride + c chain_stride], in theta or
+  int64_t group_stride, chain_stride;   // in its transposed copy
+  float* slots;                         // of the own lookup
   int own, lookups;
+};
+struct GrPasses {
+  GrPass pass[BVI_MAX_LOOKUPS];
 };
 
 // the workgroup's dense sums: [0] e^2, [1] e, [2 + j] e x_j; eight at a time through LDS
@@ -68,13 +72,19 @@ __device__ __forceinline__ void grouped_dense(double sum_sq, double sum_e, const
 // Up to 16 chains: CP chains x Q = 64 / CP rows per wave, every lane its own row with its own group's effect, so that
 // groups of a few rows keep all lanes busy.  Rows are sorted by group: Q rows of one group are added lane by lane; where
 // they are of several, log2 Q shuffles leave each one's sum in its first lane (300k rows of one chain in 100k groups 10 us
-// of 5 MB; a wave that took the groups one by one 32).  FIRST: this pass also takes the sums that need
-// every row once.
-template <int CP, int D, bool GRAD, bool FIRST>
-__global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
-    GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
-    const float* __restrict__ zown, int64_t n, int d, int64_t span, int C, int64_t P, const float* __restrict__ theta,
-    const float* __restrict__ tables, float* __restrict__ slots, double* __restrict__ dense) {
+// of 5 MB; a wave that took the groups one by one 32).  blockIdx.z: the lookup whose pass this is; the first also takes the
+// sums that need every row once.
+template <int CP, int D, bool GRAD>
+__global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPasses passes, int64_t n, int d, int64_t span, int C,
+                                                                int64_t P, const float* __restrict__ theta,
+                                                                double* __restrict__ dense) {
+  const GrPass& a = passes.pass[blockIdx.z];
+  const bool FIRST = blockIdx.z == 0;
+  const float* __restrict__ y = a.y;
+  const float* __restrict__ X = a.X;
+  const int32_t* __restrict__ key = a.id[a.own];
+  const float* __restrict__ zown = a.z[a.own];
+  float* __restrict__ slots = a.slots;
   constexpr int Q = 64 / CP;
   constexpr int DD = D ? D : 1;
   constexpr int U = D <= 16 ? 4 : 1;                       // rows per lane in flight
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
     auto at = [&](int t) { return i0 + t * Q + q < end ? i0 + t * Q + q : end - 1; };
     auto effect = [&](int g) {
       if (g < 0 || g >= rows) g = 0;                       // not used
-      return tables ? tables[(a.at[own] + g) * C + c] : th[a.offset[own] + g];
+      return a.tab[own][g * a.group_stride + c * a.chain_stride];
     };
     float x[U][DD], yt[U];                                 // every row's loads leave before the first is waited for
 #pragma unroll
@@ -146,7 +156,8 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(
       for (int l = 0; l < a.lookups; ++l) {
         if (l == own) continue;
         const int64_t m = a.id[l][i];
-        if (m >= 0 && m < a.rows[l]) r -= tables[(a.at[l] + m) * C + c] * (a.z[l] ? a.z[l][i] : 1.f);
+        if (m >= 0 && m < a.rows[l])
+          r -= a.tab[l][m * a.group_stride + c * a.chain_stride] * (a.z[l] ? a.z[l][i] : 1.f);
       }
 #pragma unroll
       for (int j = 0; j < D; ++j) r = fmaf(-w[j], x[t][j], r);
@@ -217,8 +228,7 @@ template <int D, bool GRAD, bool FIRST, int OTHERS>
 __global__ __launch_bounds__(64 * GR_WAVES) void grouped_wide_kernel(
     GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
     const float* __restrict__ zown, const int32_t* __restrict__ start, int64_t n, int d, int64_t span, int C, int64_t P,
-    const float* __restrict__ theta, const float* __restrict__ tables, float* __restrict__ slots,
-    double* __restrict__ dense) {
+    const float* __restrict__ theta, float* __restrict__ slots, double* __restrict__ dense) {
   constexpr int K = D <= 16 ? 2 : 1, CL = 64 / K, DD = D ? D : 1;
   constexpr int GR_TILE = D <= 16 ? 32 : 16;
   constexpr int XV = D ? (GR_TILE * D + 255) / 256 : 1;           // 16-byte loads per lane and tile
@@ -257,7 +267,7 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_wide_kernel(
     auto effect = [&](int v, float (&to)[K]) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        to[k] = tables ? tables[(a.at[own] + v) * C + c[k]] : theta[(int64_t)c[k] * P + a.offset[own] + v];
+        to[k] = a.tab[own][v * a.group_stride + c[k] * a.chain_stride];
     };
     auto look_ahead = [&]() {
       next_end = g + 1 < rows ? (int64_t)start[g + 2] : -1;
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_wide_kernel(
               const float zl = a.z[l] ? a.z[l][i0 + r] : 1.f;
 #pragma unroll
               for (int k = 0; k < K; ++k) {
-                const float t = tables[(a.at[l] + (has ? m : 0)) * C + c[k]];
+                const float t = a.tab[l][(has ? m : 0) * a.group_stride + c[k] * a.chain_stride];
                 e[k] = has ? fmaf(-t, zl, e[k]) : e[k];
               }
             }
@@ -623,6 +633,8 @@ int64_t span_of(int64_t n) {
 int64_t waves_of(int64_t n) { const int64_t s = span_of(n); return n > 0 ? (n + s - 1) / s : 1; }
 int64_t blocks_of(int64_t n) { return (waves_of(n) + GR_WAVES - 1) / GR_WAVES; }
 
+bool transposes(int lookups, int C);
+
 // 4-byte words of the workspace: the dense sums, the transposed tables, the slots of every lookup
 struct Space {
   int64_t dense, tables, slots[BVI_MAX_LOOKUPS], all;
@@ -633,7 +645,7 @@ Space space(int64_t n, int d, int lookups, const int64_t* rows, int C) {
   t.dense = at; at += words(2 * blocks_of(n) * (2 + d) * C);
   int64_t sum = 0;
   for (int l = 0; l < lookups; ++l) sum += rows[l];
-  t.tables = at; at += lookups > 1 ? words(sum * C) : 0;
+  t.tables = at; at += transposes(lookups, C) ? words(sum * C) : 0;
   for (int l = 0; l < lookups; ++l) {
     t.slots[l] = at;
     at += words((rows[l] + GR_WAVES * blocks_of(n)) * C);
@@ -642,40 +654,59 @@ Space space(int64_t n, int d, int lookups, const int64_t* rows, int C) {
   return t;
 }
 
-template <int CP, int D, bool GRAD, bool FIRST>
-void launch_pass(const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P, const float* theta,
-                 const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
-  if constexpr (CP == 64) {
-    const dim3 grid(blocks, bvi_ceil_div(C, CP));
-#define GR_WIDE(N)                                                                                                     \
-  hipLaunchKernelGGL((grouped_wide_kernel<D, GRAD, FIRST, N>), grid, dim3(64 * GR_WAVES), 0, s, a, a.y, a.X, a.id[a.own], \
-                     a.z[a.own], a.start, n, d, span, C, P, theta, tables, slots, dense)
-    if (a.lookups == 1) GR_WIDE(0);
-    else if (a.lookups == 2) GR_WIDE(1);
-    else GR_WIDE(2);
-#undef GR_WIDE
-    return;
-  }
-  hipLaunchKernelGGL((grouped_kernel<CP, D, GRAD, FIRST>), dim3(blocks, bvi_ceil_div(C, CP)), dim3(64 * GR_WAVES), 0, s, a,
-                     a.y, a.X, a.id[a.own], a.z[a.own], n, d, span, C, P, theta, tables, slots, dense);
-}
+struct GrCall {
+  GrPasses passes;
+  int64_t n, span, P;
+  int d, lookups, C, blocks;
+  const float* theta;
+  double* dense;
+  hipStream_t s;
+};
+
+// up to 16 chains: every lookup's pass in one launch
 template <int CP, int D>
-void launch_pass_mode(bool grad, bool first, const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P,
-                      const float* theta, const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
-  if (!grad) launch_pass<CP, D, false, true>(a, n, d, span, C, P, theta, tables, slots, dense, blocks, s);
-  else if (first) launch_pass<CP, D, true, true>(a, n, d, span, C, P, theta, tables, slots, dense, blocks, s);
-  else launch_pass<CP, D, true, false>(a, n, d, span, C, P, theta, tables, slots, dense, blocks, s);
+void launch_narrow(const GrCall& c, bool grad) {
+  const dim3 grid(c.blocks, bvi_ceil_div(c.C, CP), grad ? c.lookups : 1);
+  if (grad)
+    hipLaunchKernelGGL((grouped_kernel<CP, D, true>), grid, dim3(64 * GR_WAVES), 0, c.s, c.passes, c.n, c.d, c.span, c.C, c.P,
+                       c.theta, c.dense);
+  else
+    hipLaunchKernelGGL((grouped_kernel<CP, D, false>), grid, dim3(64 * GR_WAVES), 0, c.s, c.passes, c.n, c.d, c.span, c.C,
+                       c.P, c.theta, c.dense);
 }
-template <int CP>
-void launch_pass_d(int D, bool grad, bool first, const GrPass& a, int64_t n, int d, int64_t span, int C, int64_t P,
-                   const float* theta, const float* tables, float* slots, double* dense, int blocks, hipStream_t s) {
-#define GR_D(X) \
-  case X: launch_pass_mode<CP, X>(grad, first, a, n, d, span, C, P, theta, tables, slots, dense, blocks, s); break
-  switch (D) {
-    GR_D(0); GR_D(1); GR_D(2); GR_D(4); GR_D(8); GR_D(16); GR_D(32); GR_D(64);
+
+// more: their passes are long enough, and those after the first do less
+template <int D, bool GRAD, bool FIRST>
+void launch_wide_pass(const GrCall& c, const GrPass& a) {
+  const dim3 grid(c.blocks, bvi_ceil_div(c.C, 64));
+#define GR_WIDE(N)                                                                                                    \
+  hipLaunchKernelGGL((grouped_wide_kernel<D, GRAD, FIRST, N>), grid, dim3(64 * GR_WAVES), 0, c.s, a, a.y, a.X,          \
+                     a.id[a.own], a.z[a.own], a.start, c.n, c.d, c.span, c.C, c.P, c.theta, a.slots, c.dense)
+  if (a.lookups == 1) GR_WIDE(0);
+  else if (a.lookups == 2) GR_WIDE(1);
+  else GR_WIDE(2);
+#undef GR_WIDE
+}
+template <int D>
+void launch_wide(const GrCall& c, bool grad) {
+  if (!grad) return launch_wide_pass<D, false, true>(c, c.passes.pass[0]);
+  launch_wide_pass<D, true, true>(c, c.passes.pass[0]);
+  for (int l = 1; l < c.lookups; ++l) launch_wide_pass<D, true, false>(c, c.passes.pass[l]);
+}
+
+template <int D>
+void launch_passes(const GrCall& c, bool grad) {
+  switch (chain_lanes(c.C)) {
+    case 1: return launch_narrow<1, D>(c, grad);
+    case 4: return launch_narrow<4, D>(c, grad);
+    case 16: return launch_narrow<16, D>(c, grad);
+    default: return launch_wide<D>(c, grad);
   }
-#undef GR_D
 }
+// whether the tables are copied to [group, chain] first: a row's own entry comes once per group, those of other lookups
+// by gathers of a line per chain (300001 rows, 20000 and 60 groups, 4 chains: the passes take 25 us beside a copy of 5 and
+// 23 without it)
+bool transposes(int lookups, int C) { return lookups > 1 && C > 4; }
 
 }  // namespace
 
@@ -763,44 +794,46 @@ int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, c
   for (int l = 0; l < n_lookups; ++l) P += rows[l];
   float* w = (float*)ws;
   double* dense = (double*)(w + t.dense);
-  const float* tables = nullptr;
-  if (n_lookups > 1) {
-    tables = w + t.tables;
+  const bool copy = transposes(n_lookups, C);
+  if (copy)
     hipLaunchKernelGGL(grouped_transpose_kernel, dim3((unsigned)((P - d - 2 + 63) / 64), bvi_ceil_div(C, 64)), dim3(256), 0,
                        s, theta, P, (int64_t)(d + 2), P - d - 2, C, w + t.tables);
-  }
+  GrCall call;
+  call.n = n;
+  call.span = span;
+  call.P = P;
+  call.d = d;
+  call.lookups = n_lookups;
+  call.C = C;
+  call.blocks = blocks;
+  call.theta = theta;
+  call.dense = dense;
+  call.s = s;
   GrFinish f;
   f.lookups = n_lookups;
   const float* base = (const float*)packed;
   int64_t tiles = 0;
   for (int l = 0; l < n_lookups; ++l) {
     const Layout p = layout(n, d, n_lookups, rows[l], columns);
-    if (l == 0 || grad) {
-      GrPass a;
-      a.y = base + p.y;
-      a.X = base + p.X;
-      a.start = (const int32_t*)(base + p.start);
-      a.own = l;
-      a.lookups = n_lookups;
-      int64_t at = 0;
-      for (int k = 0; k < n_lookups; ++k) {
-        a.id[k] = (const int32_t*)(base + p.id[k]);
-        a.z[k] = p.z[k] >= 0 ? base + p.z[k] : nullptr;
-        a.rows[k] = rows[k];
-        a.offset[k] = d + 2 + at;
-        a.at[k] = at;
-        at += rows[k];
-      }
-      float* slots = w + t.slots[l];
-#define GR_CP(X)                                                                                                      \
-  case X:                                                                                                             \
-    launch_pass_d<X>(padded_d(d), grad != nullptr, l == 0, a, n, d, span, C, P, theta, tables, slots, dense, blocks, s); \
-    break
-      switch (cp) { GR_CP(1); GR_CP(4); GR_CP(16); GR_CP(64); }
-#undef GR_CP
+    GrPass& a = call.passes.pass[l];
+    a.y = base + p.y;
+    a.X = base + p.X;
+    a.start = (const int32_t*)(base + p.start);
+    a.slots = w + t.slots[l];
+    a.own = l;
+    a.lookups = n_lookups;
+    a.group_stride = copy ? C : 1;
+    a.chain_stride = copy ? 1 : P;
+    int64_t at = 0;
+    for (int k = 0; k < n_lookups; ++k) {
+      a.id[k] = (const int32_t*)(base + p.id[k]);
+      a.z[k] = p.z[k] >= 0 ? base + p.z[k] : nullptr;
+      a.rows[k] = rows[k];
+      a.tab[k] = copy ? w + t.tables + at * C : theta + d + 2 + at;
+      at += rows[k];
     }
-    f.start[l] = (const int32_t*)(base + p.start);
-    f.slots[l] = w + t.slots[l];
+    f.start[l] = a.start;
+    f.slots[l] = a.slots;
     f.rows[l] = rows[l];
     f.offset[l] = d + 2 + sum;
     sum += rows[l];
@@ -808,6 +841,12 @@ int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, c
     f.tile_end[l] = tiles;
     base += p.all;
   }
+#define GR_D(X) \
+  case X: launch_passes<X>(call, grad != nullptr); break
+  switch (padded_d(d)) {
+    GR_D(0); GR_D(1); GR_D(2); GR_D(4); GR_D(8); GR_D(16); GR_D(32); GR_D(64);
+  }
+#undef GR_D
   const dim3 grid((unsigned)(count + (grad ? tiles : 0)), bvi_ceil_div(C, cp));
 #define GR_CP(X)                                                                                                   \
   case X:                                                                                                          \
