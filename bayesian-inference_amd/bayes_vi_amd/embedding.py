@@ -56,7 +56,8 @@ class LookupPlan:
 
 def lookup_grad(grad_out, ids, num_rows, scale=1.0, plan=None):
     """The table's gradient [num_rows, width] (or [num_rows] for grad_out of the ids' own shape): row r is `scale` times
-    the sum of grad_out's rows whose id is r.  Rows that no id asks for are zero.  The sum's order is fixed by the ids."""
+    the sum of grad_out's rows whose id is r.  Rows that no id asks for are zero.  The sum's order is fixed by the
+    ids, the sizes and the operands' alignment: the same call gives the same bits."""
     if not isinstance(grad_out, torch.Tensor):
         raise TypeError('grad_out must be a tensor, got %s' % type(grad_out).__name__)
     _check_ids(ids, grad_out.device)

@@ -238,14 +238,16 @@ class GroupedRegression(FusedLogLikelihood):
 
     def _call(self, theta, logp, grad, relative=False):
         _native._check_f32_cuda(theta)
-        if theta.dim() != 2 or theta.shape[1] != self.n_params:
-            raise ValueError('theta must be [chains, %d], got %s' % (self.n_params, tuple(theta.shape)))
+        if theta.dim() != 2 or theta.shape[1] != self.n_params or theta.device != self.packed.device:
+            raise ValueError('theta must be [chains, %d] on %s, got %s on %s'
+                             % (self.n_params, self.packed.device, tuple(theta.shape), theta.device))
         c = theta.shape[0]
-        # scratch of this call: a captured graph keeps its own, whatever later calls need
-        buf = _native._scratch(_native.grouped_ws_bytes(self.n, self.d, self.rows, c), self.device)
-        _launch(_native.lib().bvi_grouped_logp_grad, _native._ptr(self.packed), self.n, self.d, len(self.rows), self._sizes,
-                self.mask, _native._ptr(theta), c, _native._ptr(logp), _native._ptr(grad), self._ref(relative),
-                _native._ptr(buf), buf.numel(), _native._stream())
+        with _native._Here(theta.device) as stream:
+            # scratch of this call: a captured graph keeps its own, whatever later calls need
+            buf = _native._scratch(_native.grouped_ws_bytes(self.n, self.d, self.rows, c), theta.device)
+            _launch(_native.lib().bvi_grouped_logp_grad, _native._ptr(self.packed), self.n, self.d, len(self.rows),
+                    self._sizes, self.mask, _native._ptr(theta), c, _native._ptr(logp), _native._ptr(grad),
+                    self._ref(relative), _native._ptr(buf), buf.numel(), stream)
 
 
 class GaussianMixture1D(FusedLogLikelihood):

@@ -41,8 +41,17 @@ class _MappedLikelihood(ShardedLogLikelihood):
         self.identity = bool((idx == torch.arange(n_model_params)).all()) if len(idx) == n_model_params else False
         self.valid = (idx >= 0).to(self.device)
         self.gather = idx.clamp_min(0).to(self.device)
-        self.vidx = torch.nonzero(idx >= 0).reshape(-1).to(self.device)
-        self.target_cols = idx[idx >= 0].to(self.device)
+        # a parameter that the likelihood uses in several places (a table looked up by two columns) has several kernel
+        # parameters: one index_add per use, since within one the order of the additions is not fixed
+        at, seen = [[]], {}
+        for k, c in enumerate(idx.tolist()):
+            if c >= 0:
+                use = seen[c] = seen.get(c, -1) + 1
+                if use == len(at):
+                    at.append([])
+                at[use].append(k)
+        at = [torch.tensor(k, dtype=torch.long) for k in at]
+        self.uses = [(idx[k].to(self.device), k.to(self.device)) for k in at]
 
     @property
     def logp_ref(self):
@@ -61,7 +70,8 @@ class _MappedLikelihood(ShardedLogLikelihood):
         if not want_grad:
             return lp, None
         g = torch.zeros_like(theta)
-        g.index_add_(1, self.target_cols, gk.index_select(1, self.vidx))
+        for cols, at in self.uses:
+            g.index_add_(1, cols, gk.index_select(1, at))
         return lp, g
 
 

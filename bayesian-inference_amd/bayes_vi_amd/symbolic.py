@@ -192,14 +192,16 @@ def gather(params, indices):
 def whole_numbers(column):
     """A feature column of group numbers as int64 (columns made from a data frame are float32)."""
     import torch
-    if column.dtype in (torch.int32, torch.int64):
+    if column.dtype in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
         return column.long()
     if column.is_floating_point():
         ids = column.long()
         if bool((ids.to(column.dtype) != column).any()):
             raise ValueError('a column of group numbers holds values that are not whole')
-        if column.dtype == torch.float32 and ids.numel() and int(ids.abs().max()) > 1 << 24:
-            raise ValueError('group numbers beyond 2^24 are not exact in float32: give the column as integers')
+        exact = int(2 / torch.finfo(column.dtype).eps)
+        if ids.numel() and int(ids.abs().max()) > exact:
+            raise ValueError('group numbers beyond 2^%d are not exact in %s: give the column as integers'
+                             % (exact.bit_length() - 1, str(column.dtype).replace('torch.', '')))
         return ids
     raise TypeError('a column of group numbers must hold integers, got %s' % column.dtype)
 

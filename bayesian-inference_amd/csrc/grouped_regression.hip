@@ -72,8 +72,8 @@ __device__ __forceinline__ void grouped_dense(double sum_sq, double sum_e, const
 // Up to 16 chains: CP chains x Q = 64 / CP rows per wave, every lane its own row with its own group's effect, so that
 // groups of a few rows keep all lanes busy.  Rows are sorted by group: Q rows of one group are added lane by lane; where
 // they are of several, log2 Q shuffles leave each one's sum in its first lane (300k rows of one chain in 100k groups 10 us
-// of 5 MB; a wave that took the groups one by one 32).  blockIdx.z: the lookup whose pass this is; the first also takes the
-// sums that need every row once.
+// of 5 MB; a wave that took the groups one by one 32).  300001 rows, 3 features, 4 chains, two lookups: 22 us, shuffles and
+// gathers, not bytes.  blockIdx.z: the lookup whose pass this is; the first also takes the sums that need every row once.
 template <int CP, int D, bool GRAD>
 __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPasses passes, int64_t n, int d, int64_t span, int C,
                                                                 int64_t P, const float* __restrict__ theta,
@@ -220,10 +220,10 @@ __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPasses passes,
 
 // 64 chains per wave: 32 lanes of two chains each times two rows.  A wave keeps 32 rows in LDS (its own part: no
 // barriers) and has the next ones on their way in registers, long enough to hide their latency; a row's features are then
-// read by broadcast, once for two chains.  What remains is 2 D + 3 vector instructions per row and chain.  Read straight
-// from memory through scalar loads, rows cost 81 us at 1M rows, D = 8, 64 chains; with the next block of scalars on its
-// way too many registers (93 us).  OTHERS: tables beside the own one (2: any number beyond one).
-// Beyond 16 features a lane has registers for one chain, and the tile is 16 rows.
+// read by broadcast, once for two chains.  What remains is 2 D + 3 vector instructions per row and chain, 35 us of the 54
+// that 1M rows, D = 8, 64 chains take.  Read straight from memory through scalar loads, rows cost 81 us there; with the
+// next block of scalars on its way too many registers (93 us).  OTHERS: tables beside the own one (2: any number beyond
+// one).  Beyond 16 features a lane has registers for one chain, and the tile is 16 rows.
 template <int D, bool GRAD, bool FIRST, int OTHERS>
 __global__ __launch_bounds__(64 * GR_WAVES) void grouped_wide_kernel(
     GrPass a, const float* __restrict__ y, const float* __restrict__ X, const int32_t* __restrict__ key,
@@ -565,14 +565,15 @@ __global__ __launch_bounds__(256) void grouped_pack_kernel(const float* __restri
   for (int j = 0; j < D; ++j) Xo[i * D + j] = j < d ? X[k * d + j] : 0.f;
 }
 __global__ __launch_bounds__(256) void grouped_pack_column_kernel(const int32_t* __restrict__ id,
-                                                                  const float* __restrict__ z, int64_t n,
+                                                                  const float* __restrict__ z, int64_t rows, int64_t n,
                                                                   const int32_t* __restrict__ order,
                                                                   int32_t* __restrict__ ido, float* __restrict__ zo) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n) return;
   const int64_t k = order[i];
-  ido[i] = id[k];
-  if (zo) zo[i] = z[k];
+  const int32_t g = id[k];
+  ido[i] = g;
+  if (zo) zo[i] = g >= 0 && g < rows ? z[k] : 0.f;       // what stands beside no group is not a number to multiply with
 }
 __global__ __launch_bounds__(256) void grouped_pack_start_kernel(const int32_t* __restrict__ start, int64_t m,
                                                                  int32_t* __restrict__ out) {
@@ -760,7 +761,7 @@ int bvi_grouped_pack(const float* X, const float* y, int64_t n, int d, int n_loo
                          base + t.y);
       for (int k = 0; k < n_lookups; ++k)
         hipLaunchKernelGGL(grouped_pack_column_kernel, grid, dim3(256), 0, s, ids[k],
-                           t.z[k] >= 0 ? columns[k] : nullptr, n, order, (int32_t*)(base + t.id[k]),
+                           t.z[k] >= 0 ? columns[k] : nullptr, rows[k], n, order, (int32_t*)(base + t.id[k]),
                            t.z[k] >= 0 ? base + t.z[k] : nullptr);
     }
     base += t.all;

@@ -496,9 +496,9 @@ int bvi_lookup_grad(const void* grad_out, int dtype, int64_t n, int64_t width, i
 
 /* ---- Gaussian linear regression with group-level effects: the loss that reads such tables, with its gradient.
  *   y_i ~ Normal(b + x_i . w + sum_l z_il u_l[ids_l[i]], s);  theta = (b, w[d], s, u_1[rows_1], u_2[rows_2], ...)
- * z_l (columns[l]) may be NULL: ones.  An id outside [0, rows_l) has no effect.  d <= 64, n_lookups <=
- * BVI_MAX_LOOKUPS, all tables together at most 2^25 rows.  `rows`, `ids` and `columns` (arrays of n_lookups) are HOST arrays; `ids[l]` and
- * `columns[l]` device pointers.  bvi_grouped_pack lays the rows out once per dataset, in every lookup's order;
+ * z_l (columns[l]) may be NULL: ones.  An id outside [0, rows_l) has no effect, whatever z_l holds there.  d <= 64,
+ * n_lookups <= BVI_MAX_LOOKUPS, all tables together at most 2^25 rows.  `rows`, `ids` and `columns` (arrays of
+ * n_lookups) are HOST arrays; `ids[l]` and `columns[l]` device pointers.  bvi_grouped_pack lays the rows out once per dataset, in every lookup's order;
  * `columns` of the other calls has bit l set where columns[l] was given.  Conventions of logp, grad, logp_ref and shards
  * as for the families above. */
 #define BVI_MAX_LOOKUPS 8

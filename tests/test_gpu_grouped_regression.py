@@ -224,6 +224,63 @@ def test_rows_without_a_group_have_no_effect(gpu_device):
         assert (np.abs(g.cpu().numpy() - rg[:, keep]) <= bg[:, keep]).all()
 
 
+@pytest.mark.parametrize('chains', [1, 3, 16, 40])
+@pytest.mark.parametrize('n_lookups', [1, 2])
+def test_columns_beside_no_group_are_not_used(gpu_device, n_lookups, chains):
+    """What a multiplier holds in rows without a group of its lookup (here NaN and infinities) changes nothing."""
+    from bayes_vi_amd import _native as nat
+    rng, groups = np.random.default_rng(10), [9, 5][:n_lookups]
+    X, y, ids, z, theta = make(rng, 700, 1, groups, chains)
+    z = [rng.normal(size=700).astype(np.float32) for _ in groups]
+    masked = []
+    for i, k, rows in zip(ids, z, groups):
+        out = rng.random(700) < 0.3
+        i[out] = rng.choice([-1, rows, 2 ** 31 - 1], out.sum())
+        masked.append(k.copy())
+        masked[-1][out] = rng.choice([np.nan, np.inf, -np.inf], out.sum())
+        k[out] = 0.0
+    dev = lambda a: torch.tensor(a, device=gpu_device)
+    th, got = dev(theta), []
+    for columns in (z, masked):
+        packed, mask = nat.grouped_pack(dev(X), dev(y), [dev(i.astype(np.int32)) for i in ids], groups, [dev(k) for k in columns])
+        lp, g = torch.empty(chains, device=gpu_device), torch.empty_like(th)
+        ws = nat._scratch(nat.grouped_ws_bytes(700, 1, groups, chains), gpu_device)
+        nat.check(nat.lib().bvi_grouped_logp_grad(packed.data_ptr(), 700, 1, n_lookups, nat._int64s(groups), mask,
+                                                  th.data_ptr(), chains, lp.data_ptr(), g.data_ptr(), None, ws.data_ptr(),
+                                                  ws.numel(), nat._stream()), 'bvi_grouped_logp_grad')
+        got.append((lp, g))
+    assert torch.isfinite(got[0][0]).all() and torch.isfinite(got[0][1]).all()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_a_table_looked_up_three_times(gpu_device):
+    """One table of a model read by three columns: the gradient is the sum over the uses, the same bits every time."""
+    import bayes_vi_amd.distributions as tfd
+    from bayes_vi_amd import symbolic as sym
+    from bayes_vi_amd.model import Model
+    rng, G, n = np.random.default_rng(11), 300, 5000
+    ids = [rng.integers(0, G, n) for _ in range(3)]
+    y = rng.normal(size=n).astype(np.float32)
+    priors = collections.OrderedDict(u=tfd.Normal(torch.zeros(G), torch.ones(G)), scale=tfd.HalfNormal(2.))
+    model = Model(priors, lambda u, scale, features: tfd.Normal(
+        loc=sym.gather(u, features['a']) + sym.gather(u, features['b']) - sym.gather(u, features['c']), scale=scale))
+    feats = {k: torch.tensor(i, device=gpu_device) for k, i in zip('abc', ids)}
+    lik = model._build_likelihood(feats, torch.tensor(y, device=gpu_device))
+    theta = np.concatenate([rng.normal(size=(4, G)), rng.uniform(0.7, 2.0, (4, 1))], 1).astype(np.float32)
+    th = torch.tensor(theta, device=gpu_device)
+    lp, g = lik.logp_grad(th)
+    kernel_theta = np.concatenate([np.zeros((4, 1)), theta[:, G:]] + [theta[:, :G]] * 3, 1).astype(np.float32)
+    z = [None, None, -np.ones(n, np.float32)]
+    rlp, rg, blp, bg = oracle(np.zeros((n, 0), np.float32), y, ids, z, kernel_theta, [G] * 3)
+    assert (np.abs(lp.cpu().numpy() - rlp) <= blp).all()
+    fold = lambda a: np.concatenate([a[:, 2:].reshape(4, 3, G).sum(1), a[:, 1:2]], 1)
+    e, b = np.abs(g.cpu().numpy() - fold(rg)), fold(bg)
+    b += 3 * U * fold(np.abs(rg))                             # two additions of the three uses
+    assert (e <= b).all()
+    for _ in range(5):
+        assert torch.equal(lik.logp_grad(th)[1], g)
+
+
 def test_refusals(gpu_device):
     from bayes_vi_amd.fused_target import GroupedRegression
     y = torch.zeros(5, device=gpu_device)

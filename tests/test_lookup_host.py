@@ -180,3 +180,36 @@ def test_global_clipnorm_on_the_host_path():
         q.grad = torch.full_like(q, float('inf'))
     opt.step()
     assert all(torch.isnan(q).all() for q in p)
+
+
+def test_group_numbers_of_other_types():
+    """Any integers; floating-point columns as far as their type holds whole numbers exactly."""
+    for t in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
+        assert sym.whole_numbers(torch.tensor([0, 7, 3], dtype=t)).tolist() == [0, 7, 3]
+    for t, bits in ((torch.bfloat16, 8), (torch.float16, 11), (torch.float32, 24), (torch.float64, 53)):
+        assert sym.whole_numbers(torch.tensor([2.0 ** bits], dtype=t)).tolist() == [2 ** bits]
+        with pytest.raises(ValueError, match='2\\^%d are not exact' % bits):
+            sym.whole_numbers(torch.tensor([2.0 ** (bits + 1)], dtype=t))
+
+
+def test_a_table_looked_up_by_several_columns():
+    """Its gradient is the sum over the uses, in the order of the uses whatever the device does with one index_add."""
+    from bayes_vi_amd.model.model import _MappedLikelihood
+
+    class Inner:
+        device, group, sharded, logp_ref = torch.device('cpu'), None, False, None
+
+        def logp_grad(self, theta, want_grad=True, relative=False):
+            self.theta = theta
+            return theta.sum(1), torch.tensor([[1.0, 2.0 ** 24, 3.0, 1.0, 7.0, 1.0, 9.0, 1.0]])
+
+    feats = dict(a=torch.zeros(6), b=torch.zeros(6), c=torch.zeros(6))
+    m = Model(_priors(u=2, scale=0), lambda u, scale, features: tfd.Normal(
+        loc=sym.gather(u, features['a']) + sym.gather(u, features['b']) - sym.gather(u, features['c']), scale=scale))
+    index = m.describe_likelihood(feats)['index']
+    assert index == [-1, 2, 0, 1, 0, 1, 0, 1]
+    lik = _MappedLikelihood(Inner(), index, 3)
+    assert [cols.tolist() for cols, _ in lik.uses] == [[2, 0, 1], [0, 1], [0, 1]]
+    lp, g = lik.logp_grad(torch.tensor([[4.0, 5.0, 6.0]]))
+    assert lik.inner.theta.tolist() == [[0.0, 6.0, 4.0, 5.0, 4.0, 5.0, 4.0, 5.0]]
+    assert g.tolist() == [[3.0 + 7.0 + 9.0, 3.0, 2.0 ** 24]]
