@@ -72,7 +72,7 @@ __device__ __forceinline__ void grouped_dense(double sum_sq, double sum_e, const
 // Up to 16 chains: CP chains x Q = 64 / CP rows per wave, every lane its own row with its own group's effect, so that
 // groups of a few rows keep all lanes busy.  Rows are sorted by group: Q rows of one group are added lane by lane; where
 // they are of several, log2 Q shuffles leave each one's sum in its first lane (300k rows of one chain in 100k groups 10 us
-// of 5 MB; a wave that took the groups one by one 32).  300001 rows, 3 features, 4 chains, two lookups: 22 us, shuffles and
+// of 5 MB; a wave that took the groups one by one 32).  300001 rows, 3 features, 4 chains, two lookups: 24 us, shuffles and
 // gathers, not bytes.  blockIdx.z: the lookup whose pass this is; the first also takes the sums that need every row once.
 template <int CP, int D, bool GRAD>
 __global__ __launch_bounds__(64 * GR_WAVES) void grouped_kernel(GrPasses passes, int64_t n, int d, int64_t span, int C,

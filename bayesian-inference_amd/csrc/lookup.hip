@@ -21,7 +21,8 @@ struct alignas(sizeof(T) * V) Pack {
 // ---- forward -------------------------------------------------------------------------------------------------------
 // One thread moves one vector of V elements; tc threads side by side hold one row's columns (all of them up to 256,
 // else equal parts), 256 / tc rows per step, four steps' ids and vectors in flight.  Nothing but bytes: 65537 rows of 640
-// bf16 out of 100003 take 26 us, 6.4 TB/s of reads and writes; 919 x 4 are the launch, 3 us.
+// bf16 out of 100003 take 32 us from memory, 5.2 TB/s of reads and writes (26 where a cache holds some of the table);
+// 919 x 4 are the launch, 3 us.
 constexpr int LK_UNROLL = 4;
 
 template <typename T, int V, typename I>

@@ -163,7 +163,7 @@ __device__ __forceinline__ double mt_factor(double norm, double clip) {
   return norm > clip ? clip / norm : 1.0;
 }
 
-// One read: 58M values, bf16 and float (216 MB), 33 us = 6.5 TB/s, as fast as this memory reads.
+// One read: 58M values, bf16 and float (216 MB), 38 us = 5.6 TB/s (33 where the caches hold some of it).
 __global__ __launch_bounds__(256) void norm_kernel(NormArgs a, double* __restrict__ part) {
   __shared__ double red[4];
   double s = 0.0;
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restri
 }
 
 // every workgroup adds up the same partial sums (at most a few KB from L2) instead of waiting for a launch that does.
-// One read and one write: the same 58M values 67 us = 6.5 TB/s.
+// One read and one write: the same 58M values 68 us = 6.4 TB/s.
 template <bool PAST_CACHE>
 __global__ __launch_bounds__(256) void clip_kernel(ClipArgs a, const double* __restrict__ part, int n_part,
                                                    const float* __restrict__ use_norm, double clip, float* __restrict__ norm_out) {
@@ -352,7 +352,7 @@ __device__ __forceinline__ void adam_update(float* __restrict__ x, float* __rest
   }
 }
 
-// Four arrays read, three or (where a factor is not one) four written: 29M variables, 937 MB, 145 us = 6.5 TB/s.  Only
+// Four arrays read, three or (where a factor is not one) four written: 29M variables, 937 MB, 144 us = 6.5 TB/s.  Only
 // bytes count; the norm pass before it is the fifth read, since every variable's norm is needed before its first step.
 __global__ __launch_bounds__(256) void adam_update_kernel(AdamArgs a, AdamHyper h, const float* __restrict__ factor,
                                                           const double* __restrict__ state) {
