@@ -343,10 +343,10 @@ __global__ __launch_bounds__(256) void sort_start_kernel(StartJob j) { start_par
 // So that no thread has many positions of one row to add: blocks of 2^chunk_bits sorted positions that belong to one row
 // are summed beforehand (level 1), blocks of 2^fan_bits of those again (level 2), and so on; a row adds the entries at
 // its ends one by one and whole blocks in between.  Two forms of the three kernels:
-//   wide rows, or few positions per row: a thread per vector of V columns, two or three positions in flight (more cost
-//   the registers of a wave that hides as much: 65537 x 640 bf16 into 100003 rows 66 us with four, 41 with two, which is
-//   5.2 TB/s; 69 where no cache holds any of the 212 MB: a row's start, its position, its vector wait for one another,
-//   and carrying three rows along in a thread's registers took 79);
+//   wide rows, or few positions per row: a thread per vector of V columns, three positions in flight
+//   (65537 x 640 bf16 into 100003 rows, 212 MB that no cache holds: 62 us, 3.4 TB/s; a row's start, its position and its
+//   vector wait for one another, yet neither positions fetched a row ahead, 62, nor four rows at a time, 82, nor three rows
+//   carried along in registers, 79, hid more than a wave more per SIMD does);
 //   narrow rows: a wave per row, LE lanes across the columns times Q = 64 / LE over the positions (2M x 16 into 5000 rows
 //   14 us after 29 us for the blocks of 128; a thread per vector took 43 after 42; waves that walk the sorted positions and
 //   read everything once 41 - 51, since a gathered row of 64 bytes costs the 128 of its line whoever reads it).
@@ -457,7 +457,9 @@ __global__ __launch_bounds__(256) void grad_level_kernel(const S* __restrict__ s
   }
 }
 
-// A thread per vector; the next row's place in the order is on its way while this one's positions are added.
+// A thread per vector; the next row's place in the order is on its way while this one's positions are added.  Vectors of
+// eight are added up in halves where a row has several positions: 64 registers instead of 86, eight waves instead of five
+// (65537 x 640 bf16 into 100003 rows 71 -> 62 us; where rows have six positions each, 300000 x 256 f16 into 50000, 53 -> 57).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, int64_t stride, int W, int tc,
                                                        const int32_t* __restrict__ order,
@@ -471,18 +473,28 @@ __global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, 
   while (true) {
     const int64_t next = r + step < rows ? r + step : r;
     const int sn = start[next], en = start[next + 1];
-    for (int col = col0; col < W; col += tc) {
-      float acc[V] = {};
-      if (e - s == 1) {                                  // most rows of a large table: one position or none
-        const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(g + order[s] * stride + (int64_t)col * V);
+    if (e - s <= 1) {                                    // most rows of a large table: one position or none
+      const T* from = g + (e > s ? order[s] * stride : 0);
+      for (int col = col0; col < W; col += tc) {
+        float acc[V] = {};
+        if (e > s) {
+          const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(from + (int64_t)col * V);
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] = (float)x.e[k] * scale;
-      } else if (e > s) {
-        grad_row_sum<T, V, 1, V == 8 ? 2 : 3>(acc, g, stride, (int64_t)col * V, order, s, e, 0, width, lv, sums);
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] *= scale;
+          for (int k = 0; k < V; ++k) acc[k] = (float)x.e[k] * scale;
+        }
+        grad_store<T, V>(out + r * width + (int64_t)col * V, acc);
       }
-      grad_store<T, V>(out + r * width + (int64_t)col * V, acc);
+    } else {
+      constexpr int H = V == 8 ? 4 : V, PARTS = V / H;
+#pragma unroll 1
+      for (int part = col0 * PARTS; part < W * PARTS; part += (part + 1) % PARTS ? 1 : (tc - 1) * PARTS + 1) {
+        const int64_t at = (int64_t)part * H;
+        float acc[H] = {};
+        grad_row_sum<T, H, 1, 3>(acc, g, stride, at, order, s, e, 0, width, lv, sums);
+#pragma unroll
+        for (int k = 0; k < H; ++k) acc[k] *= scale;
+        grad_store<T, H>(out + r * width + at, acc);
+      }
     }
     if (next == r) return;
     r = next;
