@@ -413,3 +413,41 @@ def test_row_shards_add_up(gpu_device):
     rlp, rg, blp, bg = oracle(X, y, ids, z, theta, [20, 5])
     assert (np.abs(sum(p[0].double() for p in parts).cpu().numpy() - rlp) <= 2 * blp).all()
     assert (np.abs(sum(p[1].double() for p in parts).cpu().numpy() - rg) <= 2 * bg).all()
+
+
+@pytest.mark.parametrize('chains', [16, 17, 64])
+def test_sums_over_many_rows_do_not_lose_bits(gpu_device, chains):
+    """Log-densities, and their differences between chains, at 9M rows in two groups.  y, the effects and the weights are
+    multiples of 2^-8 and the features -1, 0 or 1, so every residual is exact, |e| < 4, and e^2 a multiple of 2^-16 below 16:
+    a float holds the sum of 16 of them exactly, not that of a thousand.  Sums that move to double every 32 rows or sooner
+    therefore leave nothing but the roundings of the results (2 u each; the double arithmetic is off by 2^-52 of ~1e7),
+    however many rows there are.  Sums of e and e x are multiples of 2^-8 below 2^13 within 2048 rows: exact as well."""
+    from bayes_vi_amd.fused_target import GroupedRegression
+    n, d = 9_000_001, 2
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(chains)
+    grid = lambda t: torch.round(t * 256) / 256
+    X = torch.randint(-1, 2, (n, d), generator=gen, device=gpu_device).float()
+    ids = (torch.rand(n, generator=gen, device=gpu_device) < 0.3).long()
+    e0 = grid(torch.randn(n, generator=gen, device=gpu_device).clamp_(-3, 3))
+    w, u = torch.tensor([0.25, -0.5], device=gpu_device), torch.tensor([1.5, -0.75], device=gpu_device)
+    y = 0.5 + X @ w + u[ids] + e0
+    off = grid(0.15 * torch.rand(chains, 5, generator=gen, device=gpu_device))       # |e - e0| <= 0.6 < 1
+    th = torch.cat([0.5 + off[:, :1], w + off[:, 1:3], 1 + off[:, :1], u + off[:, 3:]], 1)
+    lik = GroupedRegression(X, y, [ids], [2])
+    y64, X64 = y.double(), X.double()
+    want, grads = [], []
+    for t in th.double():
+        e = y64 - t[0] - X64 @ t[1:3] - t[4:][ids]
+        s, sq = float(t[3]), float((e * e).sum())
+        want.append(-n * math.log(s) - n / 2 * math.log(2 * math.pi) - sq / (2 * s * s))
+        back = torch.stack([(e * (1 - ids)).sum(), (e * ids).sum()])
+        grads.append(torch.cat([e.sum()[None], e @ X64, torch.tensor([sq / s - n * s], device=gpu_device), back]).cpu() / s ** 2)
+    want, grads = np.array(want), torch.stack(grads).numpy()
+    lik.logp_ref = torch.tensor([want[0], 0.0], dtype=torch.float64, device=gpu_device)
+    rel, g = lik.logp_grad(th, relative=True)
+    err = np.abs(rel.double().cpu().numpy() - (want - want[0]))
+    assert (err <= 2 * U * np.abs(want - want[0]) + 1e-7).all(), err.max()
+    # d s is a difference of two terms of the size n / s
+    assert (np.abs(g.double().cpu().numpy() - grads) <= 2 * U * np.abs(grads) + 1e-7).all()
+    value, none = lik.logp_grad(th, want_grad=False, relative=True)
+    assert none is None and (np.abs(value.double().cpu().numpy() - (want - want[0])) <= 2 * U * np.abs(want - want[0]) + 1e-7).all()
