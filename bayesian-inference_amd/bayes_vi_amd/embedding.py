@@ -10,6 +10,7 @@ every call can be recorded into a graph.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _native
 
@@ -32,6 +33,12 @@ def _rows_view(t, what):
     if width > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < width:
         t = t.contiguous()
     return t, (t.stride(0) if rows > 1 else width)
+
+
+def _differentiated(t):
+    """Whether autograd follows t: backwards, or forwards by a tangent (which `requires_grad` says nothing about)."""
+    return (torch.is_grad_enabled() and t.requires_grad
+            or _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None)
 
 
 class LookupPlan:
@@ -57,7 +64,8 @@ class LookupPlan:
 def lookup_grad(grad_out, ids, num_rows, scale=1.0, plan=None):
     """The table's gradient [num_rows, width] (or [num_rows] for grad_out of the ids' own shape): row r is `scale` times
     the sum of grad_out's rows whose id is r.  Rows that no id asks for are zero.  The sum's order is fixed by the
-    ids, the sizes and the operands' alignment: the same call gives the same bits."""
+    ids, the sizes and the operands' alignment: the same call gives the same bits.  Linear in grad_out, and differentiable
+    in it (the derivative is the lookup)."""
     if not isinstance(grad_out, torch.Tensor):
         raise TypeError('grad_out must be a tensor, got %s' % type(grad_out).__name__)
     _check_ids(ids, grad_out.device)
@@ -68,13 +76,20 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, plan=None):
     if not flat and (grad_out.dim() != ids.dim() + 1 or grad_out.shape[:-1] != ids.shape or grad_out.shape[-1] < 1):
         raise ValueError('grad_out must have shape %s or %s + (width,), got %s'
                          % (tuple(ids.shape), tuple(ids.shape), tuple(grad_out.shape)))
+    if plan is not None:
+        plan.check(ids.numel(), num_rows, grad_out.device)
+    if _differentiated(grad_out):
+        return _LookupGrad.apply(grad_out, ids, num_rows, float(scale), plan)
+    return _gradient(grad_out, ids, num_rows, float(scale), plan)
+
+
+def _gradient(grad_out, ids, num_rows, scale, plan):
+    flat = grad_out.dim() == ids.dim()
     n, width = ids.numel(), 1 if flat else grad_out.shape[-1]
     g, stride = _rows_view(grad_out.reshape(n, width), 'grad_out')
-    if plan is not None:
-        plan.check(n, num_rows, g.device)
     ids = ids.contiguous()
     out = torch.empty((num_rows,) if flat else (num_rows, width), dtype=g.dtype, device=g.device)
-    _native.lookup_grad(g, n, width, stride, ids, None if plan is None else plan.buffer, num_rows, float(scale), out)
+    _native.lookup_grad(g, n, width, stride, ids, None if plan is None else plan.buffer, num_rows, scale, out)
     return out
 
 
@@ -91,6 +106,7 @@ class _Lookup(torch.autograd.Function):
     def forward(ctx, table, ids, scale, plan):
         ctx.scale, ctx.plan, ctx.rows = scale, plan, table.shape[0]
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         return _forward(table, ids, scale)
 
     @staticmethod
@@ -99,10 +115,34 @@ class _Lookup(torch.autograd.Function):
         ids, = ctx.saved_tensors
         return lookup_grad(grad_out, ids, ctx.rows, ctx.scale, ctx.plan), None, None, None
 
+    @staticmethod
+    def jvp(ctx, tangent, *_):                           # the map is linear in the table
+        ids, = ctx.saved_tensors
+        return lookup(tangent, ids, ctx.scale, ctx.plan)
+
+
+class _LookupGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad_out, ids, num_rows, scale, plan):
+        ctx.rows, ctx.scale, ctx.plan = num_rows, scale, plan
+        ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
+        return _gradient(grad_out, ids, num_rows, scale, plan)
+
+    @staticmethod
+    def backward(ctx, grad_table):
+        ids, = ctx.saved_tensors
+        return lookup(grad_table, ids, ctx.scale, ctx.plan), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        ids, = ctx.saved_tensors
+        return lookup_grad(tangent, ids, ctx.rows, ctx.scale, ctx.plan)
+
 
 def lookup(table, ids, scale=1.0, plan=None):
     """scale * table[ids]: shape ids.shape + (width,), or ids.shape for a one-dimensional table.  Differentiable once in
-    the table; `plan` (see `LookupPlan`) is used by the gradient only."""
+    the table, backwards and in forward mode; `plan` (see `LookupPlan`) is used by the gradient only."""
     if not isinstance(table, torch.Tensor) or table.dim() not in (1, 2):
         raise ValueError('table must be a tensor [rows, width] or [rows]')
     if table.shape[0] < 1 or table.shape[-1] < 1:
@@ -110,6 +150,6 @@ def lookup(table, ids, scale=1.0, plan=None):
     _check_ids(ids, table.device)
     if plan is not None:
         plan.check(ids.numel(), table.shape[0], table.device)
-    if torch.is_grad_enabled() and table.requires_grad:
+    if _differentiated(table):
         return _Lookup.apply(table, ids, float(scale), plan)
     return _forward(table, ids, float(scale))

@@ -296,3 +296,57 @@ def test_offsets_beyond_32_bits(emb, gpu_device):
     g[-1] = 4.0
     got = emb.lookup_grad(g, ids, 2)
     assert bool((got[0] == torch.tensor(n - 3., device=gpu_device).bfloat16()).all()) and bool((got[1] == 6.0).all())
+
+
+def test_forward_mode(emb, gpu_device):
+    """A tangent of the table goes through the lookup as the table itself does: jvp(lookup) = lookup(tangent)."""
+    import torch.autograd.forward_ad as fwd
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(12)
+    ids = torch.randint(-1, 7, (9, 5), generator=gen, device=gpu_device)
+    for shape in ((6, 4), (6,)):
+        table, tangent = (torch.randn(*shape, generator=gen, device=gpu_device) for _ in range(2))
+        want, dwant = emb.lookup(table, ids, scale=0.5), emb.lookup(tangent, ids, scale=0.5)
+        keep = ((ids >= 0) & (ids < 6)).reshape(ids.shape + (1,) * (len(shape) - 1))
+        assert torch.equal(dwant, torch.where(keep, 0.5 * tangent[ids.clamp(0, 5)], 0.0))
+        for grad_mode in (True, False):
+            for leaf in (True, False):
+                with fwd.dual_level(), torch.set_grad_enabled(grad_mode):
+                    t = table.clone().requires_grad_(leaf)
+                    out = fwd.unpack_dual(emb.lookup(fwd.make_dual(t, tangent), ids, scale=0.5))
+                    assert torch.equal(out.primal, want) and out.tangent is not None and torch.equal(out.tangent, dwant)
+        with fwd.dual_level():                       # an operand without a tangent has none afterwards either
+            assert fwd.unpack_dual(emb.lookup(table, ids)).tangent is None
+
+
+def test_forward_over_reverse(emb, gpu_device):
+    """The Hessian of sum(lookup(table)^3) times a vector, forwards over the gradient: 6 scale^3 count table vector."""
+    import torch.autograd.forward_ad as fwd
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(13)
+    for n in (40, 3000):                             # with and without the sort
+        ids = torch.randint(-1, 7, (n,), generator=gen, device=gpu_device)
+        table = torch.randint(-3, 4, (6, 4), generator=gen, device=gpu_device).float().requires_grad_()
+        v = torch.randint(-3, 4, (6, 4), generator=gen, device=gpu_device).float()
+        count = torch.bincount(ids[(ids >= 0) & (ids < 6)], minlength=6)[:, None].float()
+        with fwd.dual_level():
+            dual = fwd.make_dual(table, v)
+            g, = torch.autograd.grad((emb.lookup(dual, ids, scale=2.0) ** 3).sum(), dual)
+            g = fwd.unpack_dual(g)
+            # small whole numbers: exact
+            assert torch.equal(g.primal, 24 * count * table.detach() ** 2)
+            assert g.tangent is not None and torch.equal(g.tangent, 48 * count * table.detach() * v)
+
+
+def test_the_gradient_is_differentiable_in_what_it_adds_up(emb, gpu_device):
+    """lookup_grad is linear in grad_out: its derivative is the lookup, both ways."""
+    import torch.autograd.forward_ad as fwd
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(14)
+    for shape in ((50, 3), (50,)):
+        ids = torch.randint(-1, 7, (50,), generator=gen, device=gpu_device)
+        g = torch.randn(*shape, generator=gen, device=gpu_device, requires_grad=True)
+        w = torch.randn((6,) + shape[1:], generator=gen, device=gpu_device)
+        emb.lookup_grad(g, ids, 6, scale=0.5).backward(w)
+        assert torch.equal(g.grad, emb.lookup(w, ids, scale=0.5))
+        t = torch.randn(*shape, generator=gen, device=gpu_device)
+        with fwd.dual_level():
+            out = fwd.unpack_dual(emb.lookup_grad(fwd.make_dual(g.detach(), t), ids, 6, scale=0.5))
+            assert torch.equal(out.tangent, emb.lookup_grad(t, ids, 6, scale=0.5))
