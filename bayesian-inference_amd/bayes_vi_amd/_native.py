@@ -540,13 +540,23 @@ def clip_by_global_norm(tensors, outputs, clip_norm, use_norm, device):
     return norm
 
 
+def share_memory(tensors):
+    """Whether two of these contiguous tensors overlap."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 def adam_step(x, g, m, v, step_count, lr, b1, b2, eps, clip_norm, global_clip_norm):
-    """bvi_adam_step over lists of contiguous float32 tensors."""
+    """bvi_adam_step over lists of contiguous float32 tensors, no two of which overlap."""
     device = x[0].device
     with _Here(device) as st:
         sizes, a = _int64s([t.numel() for t in x]), ctypes.c_size_t(0)
         check(lib().bvi_adam_step_ws_bytes(len(x), sizes, ctypes.byref(a)), 'bvi_adam_step_ws_bytes')
         ws = _scratch(a.value, device)
-        check(lib().bvi_adam_step(len(x), _pointers(x), _pointers(g), _pointers(m), _pointers(v), sizes,
-                                  step_count.data_ptr(), lr, b1, b2, eps, clip_norm, global_clip_norm, ws.data_ptr(),
-                                  ws.numel(), st), 'bvi_adam_step')
+        status = lib().bvi_adam_step(len(x), _pointers(x), _pointers(g), _pointers(m), _pointers(v), sizes,
+                                     step_count.data_ptr(), lr, b1, b2, eps, clip_norm, global_clip_norm, ws.data_ptr(),
+                                     ws.numel(), st)
+        if status and share_memory([t for ts in (x, g, m, v) for t in ts]):
+            raise ValueError('two variables of the step, or their gradients or moments, share memory: the step over the '
+                             'list would write it twice at once')
+        check(status, 'bvi_adam_step')

@@ -82,7 +82,10 @@ class _AdamState:
                     g.mul_(torch.clamp(clip_norm / (g.norm() + 1e-30), max=1.0))
             self.step()
             return
-        if self.global_clipnorm is not None or any(p.numel() > ONE_WORKGROUP_MAX for p, _, _, _ in live):
+        listed = self.global_clipnorm is not None or any(p.numel() > ONE_WORKGROUP_MAX for p, _, _, _ in live)
+        if listed and self.global_clipnorm is None and _native.share_memory([t for row in live for t in row]):
+            listed = False        # a variable twice, or one gradient for two: one after the other, as their order says
+        if listed:
             if len({id(p) for p, _, _, _ in live}) != len(live):
                 raise ValueError('a variable is in the optimiser twice: the step over the list would write it twice at once')
             hyper = (self.lr, self.b1, self.b2, self.eps)

@@ -72,8 +72,7 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
     if inplace:
         if not all(t.is_contiguous() for t in live):
             raise ValueError('clip_by_global_norm(inplace=True) needs contiguous tensors')
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in live if t.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        if _native.share_memory(live):
             raise ValueError('clip_by_global_norm(inplace=True): two tensors of the list overlap')
         src = out = live
     else:

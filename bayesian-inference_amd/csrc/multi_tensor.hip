@@ -9,6 +9,11 @@
 // Squares are summed in double: no overflow for any float, and the order of the sum is fixed by the sizes alone.
 #include "bvi_common.h"
 
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
 namespace {
 
 constexpr int MT_MAX = 80;            // tensors per launch: the arguments stay below 4 KB
@@ -457,6 +462,19 @@ int check_list(int count, const void* const* src, const int64_t* sizes, const in
   return items_fit(count, sizes) ? BVI_OK : BVI_ERR_UNSUPPORTED;
 }
 
+// whether any two of the lists' ranges share memory: the kernels write them in no particular order
+bool shares_memory(int count, const int64_t* sizes, float* const* const (&lists)[4]) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> span;
+  span.reserve((size_t)count * 4);
+  for (float* const* list : lists)
+    for (int t = 0; t < count; ++t)
+      if (sizes[t] > 0) span.emplace_back((uintptr_t)list[t], (uintptr_t)(list[t] + sizes[t]));
+  std::sort(span.begin(), span.end());
+  for (size_t k = 1; k < span.size(); ++k)
+    if (span[k].first < span[k - 1].second) return true;
+  return false;
+}
+
 int launch_norm(int count, const void* const* src, const int64_t* sizes, const int* types, double* part, int* n_part,
                 hipStream_t s) {
   *n_part = 0;
@@ -580,6 +598,11 @@ int bvi_adam_step(int n_tensors, float* const* x, float* const* grad, float* con
   const int st = bvi_adam_step_ws_bytes(n_tensors, sizes, &need);
   if (st) return st;
   if (!ws || ws_bytes < need) return BVI_ERR_WORKSPACE;
+  try {
+    if (shares_memory(n_tensors, sizes, {x, grad, m, v})) return BVI_ERR_ARG;
+  } catch (const std::bad_alloc&) {
+    return BVI_ERR_WORKSPACE;
+  }
   const hipStream_t s = (hipStream_t)stream;
   double* state = (double*)ws;
   float* factor = (float*)((char*)ws + need) - n_tensors;

@@ -523,7 +523,8 @@ int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, c
  *                             (or NULL) receives the norm that was used.
  *   bvi_adam_step             one step over all variables: each gradient clipped to clip_norm (<= 0: not), all of them
  *                             jointly to global_clip_norm (<= 0: not), left clipped in grad, then the update of
- *                             bvi_clip_adam_step; *step_count (device double) is t - 1 on entry and t afterwards. */
+ *                             bvi_clip_adam_step; *step_count (device double) is t - 1 on entry and t afterwards.
+ *                             No two arrays of the four lists may share memory (BVI_ERR_ARG). */
 int bvi_global_norm_ws_bytes(int n_tensors, size_t* ws_bytes);
 int bvi_global_norm(int n_tensors, const void* const* tensors, const int64_t* sizes, const int* dtypes, float* norm,
                     void* ws, size_t ws_bytes, void* stream);

@@ -216,3 +216,49 @@ def test_adam_non_finite_gradient(gpu_device):
     ps[0].grad, ps[1].grad = torch.full((5,), float('nan'), device=gpu_device), torch.ones(5, device=gpu_device)
     opt.clip_and_step(1.0)
     assert all(bool(torch.isnan(p).all()) for p in ps)       # one norm for all, as tf.clip_by_global_norm signals it
+
+
+def test_a_large_variable_twice_is_stepped_twice(gpu_device):
+    """Without the joint clip a variable that is listed twice, and two variables with one gradient, are stepped one after
+    the other whatever their size: the same bits as bvi_clip_adam_step in that order."""
+    from bayes_vi_amd import _native
+    from bayes_vi_amd.inference.vi import vi
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(21)
+    n = 3 * vi.ONE_WORKGROUP_MAX + 1
+    a, b = (torch.randn(n, generator=gen, device=gpu_device) for _ in range(2))
+    g = 0.1 * torch.randn(n, generator=gen, device=gpu_device)
+    for tied in ('variable', 'gradient'):
+        p = torch.nn.Parameter(a.clone())
+        q = p if tied == 'variable' else torch.nn.Parameter(b.clone())
+        p.grad = g.clone()
+        q.grad = p.grad
+        opt = vi.Adam(learning_rate=0.05).bind([p, q])
+        xs, gg = [a.clone(), b.clone()], g.clone()
+        if tied == 'variable':
+            xs[1] = xs[0]
+        m, v = [torch.zeros_like(g) for _ in range(2)], [torch.zeros_like(g) for _ in range(2)]
+        t = torch.zeros((), dtype=torch.float64, device=gpu_device)
+        for _ in range(2):
+            opt.clip_and_step(1.0)
+            for k in range(2):
+                _native.check(_native.lib().bvi_clip_adam_step(
+                    n, _native._ptr(xs[k]), _native._ptr(gg), _native._ptr(m[k]), _native._ptr(v[k]), _native._ptr(t),
+                    1 if k == 0 else 0, 0.05, 0.9, 0.999, 1e-7, 1.0, _native._stream()), 'bvi_clip_adam_step')
+        assert float(opt.t) == 2.0 and torch.equal(p.detach(), xs[0]) and torch.equal(q.detach(), xs[1])
+        assert torch.equal(p.grad, gg) and all(torch.equal(x, y) for x, y in zip(opt.m + opt.v, m + v))
+
+
+def test_variables_that_share_memory_are_refused_by_the_joint_step(gpu_device):
+    from bayes_vi_amd.inference.vi.vi import Adam
+    base = torch.ones(20, device=gpu_device)
+    for ps in ([base[:12], base[8:]], [base[:5], base[:5]]):
+        ps = [torch.nn.Parameter(p) for p in ps]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        with pytest.raises(ValueError, match='share memory'):
+            Adam(global_clipnorm=1.0).bind(ps).clip_and_step(1.0)
+    ps = [torch.nn.Parameter(torch.ones(5, device=gpu_device)) for _ in range(2)]
+    ps[0].grad = ps[1].grad = torch.ones(5, device=gpu_device)
+    with pytest.raises(ValueError, match='share memory'):
+        Adam(global_clipnorm=1.0).bind(ps).clip_and_step(1.0)
+    assert bool((ps[0] == 1).all()) and bool((base == 1).all())

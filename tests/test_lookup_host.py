@@ -213,3 +213,20 @@ def test_a_table_looked_up_by_several_columns():
     lp, g = lik.logp_grad(torch.tensor([[4.0, 5.0, 6.0]]))
     assert lik.inner.theta.tolist() == [[0.0, 6.0, 4.0, 5.0, 4.0, 5.0, 4.0, 5.0]]
     assert g.tolist() == [[3.0 + 7.0 + 9.0, 3.0, 2.0 ** 24]]
+
+
+def test_adam_step_refuses_lists_that_share_memory():
+    """Nothing is launched: the status comes from the ranges alone.  Empty variables share nothing."""
+    lib, at = _native.lib(), lambda *a: (ctypes.c_void_p * len(a))(*a)
+    ws, big = ctypes.c_void_p(1 << 20), 1 << 30
+
+    def status(x, g, m, v, sizes):
+        return lib.bvi_adam_step(len(sizes), at(*x), at(*g), at(*m), at(*v), _native._int64s(sizes), ws, .1, .9, .999, 1e-7,
+                                 1., 1., ws, big, None)
+    base = [4096, 8192, 12288, 16384]
+    for k in range(4):
+        lists = [[b, b + 64] for b in base]
+        lists[k][1] = lists[k][0] + 16                       # 5 floats from 0, 3 from the fourth of them
+        assert status(*lists, [5, 3]) == -1
+        lists[k][1] = lists[(k + 1) % 4][0]                  # one list's array in another's
+        assert status(*lists, [5, 3]) == -1
