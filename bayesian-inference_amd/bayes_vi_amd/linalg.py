@@ -74,6 +74,8 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, inplace=False):
             raise ValueError('clip_by_global_norm(inplace=True) needs contiguous tensors')
         if _native.share_memory(live):
             raise ValueError('clip_by_global_norm(inplace=True): two tensors of the list overlap')
+        if use_norm is not None and any(_native.share_memory([t, use_norm]) for t in live):
+            raise ValueError('clip_by_global_norm(inplace=True): use_norm lies in a tensor of the list, which is written')
         src = out = live
     else:
         with torch.no_grad():

@@ -519,7 +519,7 @@ int bvi_grouped_logp_grad(const void* packed, int64_t n, int d, int n_lookups, c
  *                             (tf.linalg.global_norm)
  *   bvi_clip_by_global_norm   outputs[t] = tensors[t] * min(1, clip_norm / norm), rounded once; all NaN when the norm is
  *                             not finite (tf.clip_by_global_norm).  outputs[t] may be tensors[t]; no two outputs may
- *                             overlap.  use_norm (device float, or NULL): that norm instead of the list's own.  *norm
+ *                             overlap, nor an output another tensor or use_norm.  use_norm (device float, or NULL): that norm instead of the list's own.  *norm
  *                             (or NULL) receives the norm that was used.
  *   bvi_adam_step             one step over all variables: each gradient clipped to clip_norm (<= 0: not), all of them
  *                             jointly to global_clip_norm (<= 0: not), left clipped in grad, then the update of

@@ -262,3 +262,16 @@ def test_variables_that_share_memory_are_refused_by_the_joint_step(gpu_device):
     with pytest.raises(ValueError, match='share memory'):
         Adam(global_clipnorm=1.0).bind(ps).clip_and_step(1.0)
     assert bool((ps[0] == 1).all()) and bool((base == 1).all())
+
+
+def test_the_norm_to_use_may_not_be_written(la, gpu_device):
+    """In place, use_norm inside a tensor of the list would be read by some workgroups after others had scaled it."""
+    t = torch.full((70_000,), 3.0, device=gpu_device)
+    for norm in (t[5], t[:1], t[-1:]):
+        with pytest.raises(ValueError, match='use_norm lies'):
+            la.clip_by_global_norm([torch.ones(4, device=gpu_device), t], 1.0, use_norm=norm, inplace=True)
+    assert bool((t == 3).all())
+    out, norm = la.clip_by_global_norm([t], 1.0, use_norm=t[5])          # written apart: fine
+    assert float(norm) == 3.0 and bool((out[0] == 1).all())
+    la.clip_by_global_norm([t[:7]], 1.0, use_norm=t[7], inplace=True)    # beside the tensor: fine
+    assert bool((t[:7] == 1).all()) and bool((t[7:] == 3).all())
