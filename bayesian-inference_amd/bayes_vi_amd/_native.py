@@ -20,6 +20,7 @@ BIJ_IDENTITY, BIJ_SOFTPLUS, BIJ_EXP, BIJ_SOFTMAX_CENTERED, BIJ_FILL_SCALE_TRIL =
 PRIOR_NONE, PRIOR_NORMAL, PRIOR_HALFNORMAL, PRIOR_DIRICHLET, PRIOR_WISHART_TRIL = 0, 1, 2, 3, 4
 MAX_PARAM_BLOCKS = 16
 MAX_LOOKUPS = 8
+GROUPED_MAX_D, GROUPED_MAX_ROWS = 64, 1 << 25     # feature columns beside the lookups; rows of all tables together
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ID_TYPES = {torch.int32: 0, torch.int64: 1}
 NOALLOC_MAX_CHAINS = 256

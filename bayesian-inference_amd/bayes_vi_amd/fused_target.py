@@ -218,14 +218,17 @@ class GroupedRegression(FusedLogLikelihood):
             if X.dim() != 2 or X.shape[0] != self.n or X.device != self.y.device:
                 raise ValueError('X must be [%d, D] on %s, got %s on %s' % (self.n, self.y.device, tuple(X.shape), X.device))
         self.d = 0 if X is None else X.shape[1]
-        if self.d > 64:
-            raise ValueError('at most 64 feature columns beside the group effects, got %d' % self.d)
+        if self.d > _native.GROUPED_MAX_D:
+            raise ValueError('at most %d feature columns beside the group effects, got %d' % (_native.GROUPED_MAX_D, self.d))
+        if min(self.rows) < 1 or sum(self.rows) > _native.GROUPED_MAX_ROWS:
+            raise ValueError('tables must have at least one row each and at most %d together, got %s'
+                             % (_native.GROUPED_MAX_ROWS, self.rows))
         self.n_params = self.d + 2 + sum(self.rows)
         packed_ids = []
         for i, r in zip(ids, self.rows):
             if i.dtype not in _native.ID_TYPES or i.numel() != self.n or i.device != self.y.device:
                 raise ValueError('ids must be int32 or int64 [%d] on %s' % (self.n, self.y.device))
-            if r < 1 or (self.n and (int(i.min()) < 0 or int(i.max()) >= r)):
+            if self.n and (int(i.min()) < 0 or int(i.max()) >= r):
                 raise ValueError('group numbers must lie in [0, %d)' % r)
             packed_ids.append(i.reshape(-1).to(torch.int32).contiguous())
         z = []

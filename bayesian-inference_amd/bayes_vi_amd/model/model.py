@@ -20,7 +20,7 @@ from .. import distributions as tfd
 from .. import symbolic as sym
 from ..fused_target import (FusedLogLikelihood, GaussianMixture1D, GaussianMixtureFullCov, GroupedRegression,
                             LinearRegression, MultivariateNormalTriL, NormalIID, Posterior, ShardedLogLikelihood)
-from .._native import MAX_LOOKUPS as _MAX_LOOKUPS
+from .._native import GROUPED_MAX_D as _GROUPED_MAX_D, GROUPED_MAX_ROWS as _GROUPED_MAX_ROWS, MAX_LOOKUPS as _MAX_LOOKUPS
 from ..utils import to_ordered_dict
 
 
@@ -225,6 +225,12 @@ class Model:
                 tables = [(name, key, terms, syms[name].size) for (name, key), terms in lookups.items()]
                 if len(tables) > _MAX_LOOKUPS:
                     raise sym.UnsupportedLikelihood('at most %d gathered tables are fused' % _MAX_LOOKUPS)
+                if len(order) > _GROUPED_MAX_D:
+                    raise sym.UnsupportedLikelihood('at most %d feature columns beside gathered tables are fused, got %d'
+                                                    % (_GROUPED_MAX_D, len(order)))
+                if sum(size for _, _, _, size in tables) > _GROUPED_MAX_ROWS:
+                    raise sym.UnsupportedLikelihood('gathered tables of at most %d entries together are fused (one that '
+                                                    'two columns look up counts twice)' % _GROUPED_MAX_ROWS)
                 index = [pidx(intercept) if intercept is not None else -1] + [pidx(p) for p in order] + [off[scale.name]]
                 for name, _, _, size in tables:
                     index += range(off[name], off[name] + size)

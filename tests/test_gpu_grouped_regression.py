@@ -451,3 +451,11 @@ def test_sums_over_many_rows_do_not_lose_bits(gpu_device, chains):
     assert (np.abs(g.double().cpu().numpy() - grads) <= 2 * U * np.abs(grads) + 1e-7).all()
     value, none = lik.logp_grad(th, want_grad=False, relative=True)
     assert none is None and (np.abs(value.double().cpu().numpy() - (want - want[0])) <= 2 * U * np.abs(want - want[0]) + 1e-7).all()
+
+
+def test_the_table_sizes_are_checked_before_the_ids(gpu_device):
+    from bayes_vi_amd.fused_target import GroupedRegression
+    y, i = torch.zeros(5, device=gpu_device), torch.full((5,), 7, device=gpu_device)
+    for rows in ([1 << 24, (1 << 24) + 1], [0, 3]):
+        with pytest.raises(ValueError, match='at least one row each and at most'):
+            GroupedRegression(None, y, [i, i], rows)

@@ -230,3 +230,24 @@ def test_adam_step_refuses_lists_that_share_memory():
         assert status(*lists, [5, 3]) == -1
         lists[k][1] = lists[(k + 1) % 4][0]                  # one list's array in another's
         assert status(*lists, [5, 3]) == -1
+
+
+def test_shapes_beyond_the_kernels_are_refused_at_recognition():
+    """As other unsupported likelihoods are, not by the constructor or the C entry point once the data is there."""
+    names = ['x%d' % k for k in range(65)]
+    feats = {k: torch.zeros(6) for k in names + ['g', 'h']}
+
+    def features_beside_a_table(count):
+        priors = _priors(u=3, w=count, scale=0)
+        return Model(priors, lambda u, w, scale, features: tfd.Normal(
+            loc=sym.gather(u, features['g']) + sum(w[k] * features[names[k]] for k in range(count)), scale=scale))
+    assert len(features_beside_a_table(64).describe_likelihood(feats)['columns']) == 64
+    with pytest.raises(sym.UnsupportedLikelihood, match='64 feature columns'):
+        features_beside_a_table(65).describe_likelihood(feats)
+    m = Model(_priors(u=3, scale=0), lambda u, scale, features: tfd.Normal(
+        loc=sym.gather(u, features['g']) + sym.gather(u, features['h']), scale=scale))
+    m.block_sizes = [1 << 24, 1]
+    assert m.describe_likelihood(feats)['family'] == 'grouped'
+    m.block_sizes = [(1 << 24) + 1, 1]
+    with pytest.raises(sym.UnsupportedLikelihood, match='entries together'):
+        m.describe_likelihood(feats)
