@@ -180,7 +180,8 @@ class Model:
         'columns' = [[(feature_key, coef), ...] per slope parameter] and 'offset' =
         [(feature_key | None, coef), ...] terms to subtract from y; for 'grouped' also 'lookups' = [(feature_key of the
         group numbers, table size, [(feature_key | None, coef), ...] the multiplier) per looked-up table]."""
-        syms = {name: sym.ParamSym(name, n) for name, n in zip(self.param_names, self.block_sizes)}
+        syms = {name: sym.ParamSym(name, n, shape=shape)
+                for name, n, shape in zip(self.param_names, self.block_sizes, self.param_event_shape)}
         kwargs = dict(syms)
         if not self.is_generative_model:
             if isinstance(features, dict):

@@ -79,10 +79,11 @@ class Affine:
 
 
 class ParamSym:
-    """Stand-in for one model parameter (scalar or vector)."""
+    """Stand-in for one model parameter; `shape` is that of one draw (default: a vector of `size` entries)."""
 
-    def __init__(self, name, size, index=None):
+    def __init__(self, name, size, index=None, shape=None):
         self.name, self.size, self.index = name, size, index
+        self.shape = (size,) if shape is None else tuple(shape)
 
     def as_affine(self):
         if self.size != 1 and self.index is None:
@@ -186,6 +187,9 @@ def gather(params, indices):
         return embedding.lookup(table, ids.to(params.device)).T.reshape(tuple(params.shape[:-1]) + (ids.numel(),))
     if not isinstance(params, ParamSym) or params.index is not None or not isinstance(indices, FeatureColumn):
         raise UnsupportedLikelihood('gather(u, column) needs a whole vector parameter and one feature column')
+    if len(params.shape) != 1:      # of a scalar's draws it would select chains, of a matrix's one entry in every row
+        raise UnsupportedLikelihood('gather(u, column) needs a vector parameter, %s has shape %s'
+                                    % (params.name, params.shape))
     return Affine([((params.name, RowIndex((indices.key,))), None, 1.0)])
 
 

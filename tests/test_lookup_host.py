@@ -251,3 +251,19 @@ def test_shapes_beyond_the_kernels_are_refused_at_recognition():
     m.block_sizes = [(1 << 24) + 1, 1]
     with pytest.raises(sym.UnsupportedLikelihood, match='entries together'):
         m.describe_likelihood(feats)
+
+
+def test_gather_needs_a_vector_parameter():
+    """tf.gather over the last axis of a [2, 3] parameter gives two values per row, of a scalar's draws values of other
+    chains: neither is the table of six or of one entry that the flat layout would suggest."""
+    feats = dict(g=torch.zeros(6))
+    for prior, fine in ((tfd.Normal(torch.zeros(2, 3), torch.ones(2, 3)), False), (tfd.Normal(0., 1.), False),
+                        (tfd.Normal(torch.zeros(1, 6), torch.ones(1, 6)), False),
+                        (tfd.Normal(torch.zeros(1), torch.ones(1)), True), (tfd.Normal(torch.zeros(6), torch.ones(6)), True)):
+        m = Model(collections.OrderedDict(u=prior, scale=tfd.HalfNormal(1.)),
+                  lambda u, scale, features: tfd.Normal(loc=sym.gather(u, features['g']), scale=scale))
+        if fine:
+            assert m.describe_likelihood(feats)['family'] == 'grouped'
+        else:
+            with pytest.raises(sym.UnsupportedLikelihood, match='vector parameter'):
+                m.describe_likelihood(feats)
