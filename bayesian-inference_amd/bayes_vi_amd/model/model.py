@@ -280,8 +280,7 @@ class Model:
 
     def design_matrix(self, desc, features, targets):
         """Materialises (X[N, D], y_adjusted[N]) of a 'linreg' or 'grouped' description."""
-        raw = self._feature_column(features)
-        col = lambda k: raw(k).to(torch.float32)
+        col = self._feature_column(features, torch.float32)
         y = torch.as_tensor(targets, dtype=torch.float32).reshape(-1).clone()
         for f, c in desc['offset']:
             y = y - (c if f is None else c * col(f).to(y.device))
@@ -291,24 +290,24 @@ class Model:
         return X, y
 
     @staticmethod
-    def _feature_column(features):
-        """Column by key, in the type it was given in (group numbers may be integers)."""
+    def _feature_column(features, dtype=None):
+        """Column by key, in `dtype` or the type it was given in (group numbers may be integers).  Lists are converted
+        straight to `dtype`: on the way through the type torch would choose they may not fit (10^20) or be rounded twice."""
         if isinstance(features, dict):
-            return lambda k: torch.as_tensor(features[k]).reshape(-1)
-        fmat = torch.as_tensor(features)
+            return lambda k: torch.as_tensor(features[k], dtype=dtype).reshape(-1)
+        fmat = torch.as_tensor(features, dtype=dtype)
         fmat = fmat[:, None] if fmat.dim() == 1 else fmat
         return lambda k: fmat[:, k]
 
     def lookup_columns(self, desc, features):
         """(ids, multiplier or None) of every lookup of a 'grouped' description."""
-        raw = self._feature_column(features)
+        raw, col = self._feature_column(features), self._feature_column(features, torch.float32)
         out = []
         for key, _, terms in desc['lookups']:
             ids = sym.whole_numbers(raw(key))
             z = None
             if any(f is not None or c != 1.0 for f, c in terms) or len(terms) > 1:
-                z = sum(c * (raw(f).to(torch.float32) if f is not None else torch.ones_like(ids, dtype=torch.float32))
-                        for f, c in terms)
+                z = sum(c * (col(f) if f is not None else torch.ones_like(ids, dtype=torch.float32)) for f, c in terms)
             out.append((ids, z))
         return out
 

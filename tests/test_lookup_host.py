@@ -267,3 +267,22 @@ def test_gather_needs_a_vector_parameter():
         else:
             with pytest.raises(sym.UnsupportedLikelihood, match='vector parameter'):
                 m.describe_likelihood(feats)
+
+
+def test_feature_lists_are_converted_straight_to_float32():
+    """Whole numbers beyond 64 bits, and fractions under a default type of fewer bits, keep their float32 values."""
+    feats = dict(g=[0, 2, 1], x=[10 ** 20, 1, -3], v=[1 + 2.0 ** -20, 2.5, 3.0])
+    m = Model(_priors(u=3, w=2, scale=0), lambda u, w, scale, features: tfd.Normal(
+        loc=w[0] * features['x'] + w[1] * features['v'] + sym.gather(u, features['g']) * features['v'], scale=scale))
+    d = m.describe_likelihood(feats)
+    want = torch.tensor([[1e20, 1 + 2.0 ** -20], [1., 2.5], [-3., 3.]])
+    before = torch.get_default_dtype()
+    try:
+        for default in (torch.float32, torch.bfloat16):
+            torch.set_default_dtype(default)
+            X, y = m.design_matrix(d, feats, torch.zeros(3, dtype=torch.float32))
+            (ids, z), = m.lookup_columns(d, feats)
+            assert X.dtype == torch.float32 and torch.equal(X, want)
+            assert ids.tolist() == [0, 2, 1] and torch.equal(z, want[:, 1])
+    finally:
+        torch.set_default_dtype(before)
