@@ -180,7 +180,7 @@ def gather(params, indices):
         ids = whole_numbers(indices.reshape(-1))
         if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= params.shape[-1]):
             raise IndexError('gather: an index lies outside [0, %d)' % params.shape[-1])
-        if not params.is_cuda:                      # draws of a prior live on the host
+        if not params.is_cuda or not params.numel():   # draws of a prior live on the host; of no draws there are no values
             return params[..., ids.to(params.device)]
         from . import embedding
         table = params.reshape(-1, params.shape[-1]).T

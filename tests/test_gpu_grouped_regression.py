@@ -459,3 +459,15 @@ def test_the_table_sizes_are_checked_before_the_ids(gpu_device):
     for rows in ([1 << 24, (1 << 24) + 1], [0, 3]):
         with pytest.raises(ValueError, match='at least one row each and at most'):
             GroupedRegression(None, y, [i, i], rows)
+
+
+def test_gather_of_draws(gpu_device):
+    """Any leading shape, none and no draws among them, as indexing gives it; group numbers of another type or device."""
+    from bayes_vi_amd import symbolic as sym
+    gen = torch.Generator(device=gpu_device); gen.manual_seed(3)
+    ids = torch.tensor([4, 0, 0, 2, 1], device=gpu_device)
+    for lead in ((), (1,), (7,), (3, 5), (0,), (2, 0)):
+        u = torch.randn(*lead, 5, generator=gen, device=gpu_device)
+        for i in (ids, ids.float(), ids.cpu(), ids[:0]):
+            got = sym.gather(u, i)
+            assert torch.equal(got, u[..., i.long().to(gpu_device)]) and got.device == u.device
