@@ -16,9 +16,24 @@ def kl_reverse(logu):
 # 95 at 65536, where bvi_adam_step takes 6.4, 6.9 and 11.7
 ONE_WORKGROUP_MAX = 4096
 # unconstrained parameters up to which the gradients of the ADVI surrogates are taken in closed form on the device: every
-# workgroup of those kernels looks through all of them (a mean-field step with 102 parameters 129 us against 243 by
-# autograd, with 1002 parameters 677 against 255)
+# workgroup of those kernels looks through all of them.  us a step, closed form / autograd, for 1 and 64 samples: mean-field
+# 256 parameters 213 / 237 and 232 / 276, 300 parameters 246 / 240 and 273 / 284, 512 parameters 375 / 243 and 406 / 285;
+# full-rank 256 parameters 271 / 280 and 288 / 329, 300 parameters 354 / 280 and 345 / 308, 512 parameters 520 / 281
 FUSED_ADVI_MAX = 256
+
+
+def _graph_is_alive(params):
+    """Whether an autograd graph that leads to one of these leaves is alive: it holds the leaf's gradient accumulator, which
+    is otherwise made anew for every graph and would not know what was noted on the one before."""
+    def accumulator(p):
+        with torch.enable_grad():
+            return p.view_as(p).grad_fn.next_functions[0][0]
+
+    for p in params:
+        accumulator(p).metadata['bvi_seen'] = True
+        if accumulator(p).metadata.pop('bvi_seen', False):
+            return True
+    return False
 
 
 class _AdamState:
@@ -226,12 +241,13 @@ class VI(Inference):
         `capture_graph` (default: on for GPU runs with the built-in `Adam`): after three eager steps
         the whole step -- sampling, fused log-posterior pass, backward, clipping, optimizer update -- is
         captured once as a HIP graph and replayed, which removes the per-kernel launch cost that
-        dominates on small datasets.  The steps and their results are the same either way.  (A caller that evaluated
-        `loss()` itself beforehand must not keep that loss tensor alive into `fit`: its autograd graph pins the
-        parameters' gradient accumulators to the stream it ran on, and torch then ties the capturing stream to it.)"""
+        dominates on small datasets.  The steps and their results are the same either way.  A loss that the caller
+        evaluated beforehand and still holds keeps the parameters' gradient accumulators on the stream it ran on, and a
+        captured backward pass that waits for that stream ends the process: by default the steps then stay eager (of the
+        surrogates whose step takes a backward pass), and `capture_graph=True` raises."""
         optimizer = optimizer if optimizer is not None else Adam()
         params = [p for p in self.surrogate_posterior.parameters() if p.requires_grad]
-        on_gpu = self.device.type == 'cuda'
+        on_gpu, asked = self.device.type == 'cuda', bool(capture_graph)
         if capture_graph is None:
             # a row-sharded likelihood has a collective inside the step: that stays eager unless asked for
             lik = self.posterior.likelihood
@@ -243,6 +259,11 @@ class VI(Inference):
             opt = optimizer.bind(params, capturable=True) if capture_graph else optimizer.bind(params)
         else:
             opt = optimizer(params)
+        if capture_graph and not self._fused_advi_eligible(opt) and _graph_is_alive(params):
+            if asked:
+                raise ValueError('capture_graph: an autograd graph of the surrogate\'s parameters is still alive (a loss that '
+                                 'was evaluated before and is held somewhere); drop it, or fit without capture')
+            capture_graph = False
         losses_dev = torch.zeros(num_steps, dtype=torch.float32, device=self.device)
         bar = None
         if progress_bar:

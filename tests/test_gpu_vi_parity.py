@@ -430,3 +430,53 @@ def test_golden_advi_step_through_the_c_abi(gpu_device):
                                    atol=1e-5 * lr)
     assert float(step) == 1.0
 
+
+
+@pytest.mark.parametrize('surrogate', ['mean-field ADVI of 300 parameters', 'full-rank ADVI of 300 parameters', 'flow', 'small ADVI'])
+def test_fit_while_a_loss_is_held(bvi, gpu_device, surrogate, monkeypatch):
+    """A loss that is alive across `fit` must not reach a captured backward pass, which would end the process: the steps stay
+    eager, with the results of an eager run, and asking for the capture raises.  No graph may even be begun (the stand-in
+    below raises instead).  The closed-form step has no backward pass and is captured all the same."""
+    if '300' in surrogate:
+        rng = np.random.default_rng(90)
+        priors = collections.OrderedDict(mu=bvi.tfd.Normal(0., 10.), u=bvi.tfd.Normal(torch.zeros(298), torch.ones(298)),
+                                         scale=bvi.tfd.HalfNormal(10.))
+        model = bvi.Model(priors, lambda mu, u, scale, features: bvi.tfd.Normal(
+            loc=mu + bvi.symbolic.gather(u, features['g']), scale=scale))
+        ds = bvi.TensorDataset(dict(g=torch.tensor(rng.integers(0, 298, 1000), device=gpu_device)),
+                               torch.tensor(rng.normal(size=1000), dtype=torch.float32, device=gpu_device))
+    else:
+        model, ds, _, _ = regression(bvi, gpu_device, 1_000, 2, seed=90)
+
+    def make():
+        torch.manual_seed(3)
+        if surrogate == 'flow':
+            nd = model.flat_unconstrained_param_event_ndims
+            flow = bvi.HamiltonianFlow(nd, step_sizes=torch.nn.Parameter(torch.tensor(0.1)), num_integration_steps=1)
+            return bvi.VI(model, ds, bvi.NormalizingFlow(model=model, flow_bijector=flow, extra_ndims=nd))
+        return bvi.VI(model, ds, bvi.ADVI(model, mean_field='full' not in surrogate))
+
+    def fit(vi, **kw):
+        torch.manual_seed(4)
+        return vi.fit(optimizer=bvi.Adam(learning_rate=0.01), num_steps=12, sample_size=2,
+                      num_samples_to_approx_marginals=10, progress_bar=False, **kw)[1]
+    want = fit(make(), capture_graph=False)
+    vi = make()
+    loss = vi.loss(2)
+    if surrogate == 'small ADVI':
+        np.testing.assert_allclose(fit(vi, capture_graph=True), want, rtol=1e-5)
+        assert loss.requires_grad
+        return
+
+    class NoGraph:
+        def __init__(self, *args, **kwargs):
+            raise AssertionError('a capture was begun')
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, 'CUDAGraph', NoGraph)
+        with pytest.raises(ValueError, match='still alive'):
+            fit(vi, capture_graph=True)
+        got = fit(vi)
+    np.testing.assert_allclose(got, want, rtol=1e-5)
+    assert loss.requires_grad
+    del loss
+    np.testing.assert_allclose(fit(make(), capture_graph=True), want, rtol=1e-4)
