@@ -529,17 +529,21 @@ __global__ __launch_bounds__(256) void grad_row_wave_kernel(const T* __restrict_
 }
 
 // Few positions and rows: no sort at all.  A wave per row looks through the ids, 64 at a time, lists the positions it
-// finds in ascending order, and sums them, LE lanes across the columns times 64 / LE over the list.  919 x 4 into 85 rows:
-// 5.5 us, one launch; ranking, the start of each row and the sums are three.
-constexpr int SCAN_MAX = 2048;
+// finds in ascending order, and sums them, LE lanes across the columns times Q = 64 / LE over the list.  919 x 4 into 85
+// rows: 5.5 us, one launch; ranking, the start of each row and the sums are three.  A list of more than SCAN_ALONE rounds
+// is shared by the workgroup's four waves, and where rows are few their columns go to workgroups of their own (each looks
+// through the ids again, 4 us): 2048 positions x 1999 columns into one row 45 us, x 2000 32; by one wave alone 11 ms and 2.1.
+constexpr int SCAN_MAX = 2048, SCAN_DEEP = 4, SCAN_ALONE = 4, SCAN_BLOCKS = 512;
 template <typename T, int V, int LE, typename I>
 __global__ __launch_bounds__(256) void grad_scan_kernel(const T* __restrict__ g, int64_t stride, int W,
                                                         const I* __restrict__ ids, int n, int64_t rows, float scale,
                                                         T* __restrict__ out) {
-  constexpr int Q = 64 / LE;
+  constexpr int Q = 64 / LE, LONG = SCAN_ALONE * SCAN_DEEP * Q;
   __shared__ uint16_t lists[4][SCAN_MAX];
+  __shared__ int counts[4];
+  __shared__ float parts[3][LE * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane / LE, le = lane % LE;
-  const int64_t r = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t r0 = (int64_t)blockIdx.x * 4, r = r0 + wave;
   uint16_t* list = lists[wave];
   int found = 0;
   if (r < rows) {
@@ -558,29 +562,58 @@ __global__ __launch_bounds__(256) void grad_scan_kernel(const T* __restrict__ g,
       }
     }
   }
+  if (lane == 0) counts[wave] = found;
   __syncthreads();
-  if (r >= rows) return;
-  for (int col = le; col - le < W; col += LE) {
-    float acc[V] = {};
-    if (col < W) {
-      const T* at = g + (int64_t)col * V;
-      for (int p = q; p < found; p += 4 * Q) {
-        Pack<T, V> x[4];
+  // acc += the row's positions first, first + step, ... at one vector of columns
+  auto add = [&](float (&acc)[V], const uint16_t* of, int count, int first, int step, int col) {
+    const T* at = g + (int64_t)col * V;
+    for (int p = first; p < count; p += SCAN_DEEP * step) {
+      Pack<T, V> x[SCAN_DEEP];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (p + u * Q < found) x[u] = *reinterpret_cast<const Pack<T, V>*>(at + (int64_t)list[p + u * Q] * stride);
+      for (int u = 0; u < SCAN_DEEP; ++u)
+        if (p + u * step < count) x[u] = *reinterpret_cast<const Pack<T, V>*>(at + (int64_t)of[p + u * step] * stride);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (p + u * Q < found)
+      for (int u = 0; u < SCAN_DEEP; ++u)
+        if (p + u * step < count)
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += (float)x[u].e[k];
-      }
+          for (int k = 0; k < V; ++k) acc[k] += (float)x[u].e[k];
     }
-    grad_join<V, LE>(acc);
-    if (q == 0 && col < W) {
+  };
+  auto put = [&](int64_t row, float (&acc)[V], int count, int col) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] = found ? acc[k] * scale : 0.f;
-      grad_store<T, V>(out + (r * W + col) * V, acc);
+    for (int k = 0; k < V; ++k) acc[k] = count ? acc[k] * scale : 0.f;
+    grad_store<T, V>(out + (row * W + col) * V, acc);
+  };
+  const int col0 = blockIdx.y * LE, col_step = gridDim.y * LE;
+  if (r < rows && found <= LONG) {
+    for (int c = col0; c < W; c += col_step) {
+      const int col = c + le;
+      float acc[V] = {};
+      if (col < W) add(acc, list, found, q, Q, col);
+      grad_join<V, LE>(acc);
+      if (q == 0 && col < W) put(r, acc, found, col);
+    }
+  }
+  for (int k = 0; k < 4; ++k) {                          // the same for every thread: a row that does not exist has no list
+    const int count = counts[k];
+    if (count <= LONG) continue;
+    for (int c = col0; c < W; c += col_step) {
+      const int col = c + le;
+      float acc[V] = {};
+      if (col < W) add(acc, lists[k], count, wave * Q + q, 4 * Q, col);
+      grad_join<V, LE>(acc);
+      if (wave > 0 && q == 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j) parts[wave - 1][le * V + j] = acc[j];
+      __syncthreads();
+      if (wave == 0 && q == 0 && col < W) {
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] += parts[w][le * V + j];
+        put(r0 + k, acc, count, col);
+      }
+      __syncthreads();
     }
   }
 }
@@ -822,8 +855,10 @@ int launch_grad_le(const GradCall& c) {
 
 template <typename T, int V, int LE>
 int launch_scan_le(const GradCall& c) {
-  const dim3 grid((unsigned)((c.rows + 3) / 4));
   const int W = (int)(c.width / V);
+  // columns in workgroups of their own as long as the rows' do not fill the chip twice
+  const int64_t row_blocks = (c.rows + 3) / 4, steps = (W + (int64_t)LE - 1) / LE, wanted = SCAN_BLOCKS / row_blocks;
+  const dim3 grid((unsigned)row_blocks, (unsigned)(wanted < 1 ? 1 : wanted < steps ? wanted : steps));
   if (c.ids_type == BVI_IDS_I32)
     hipLaunchKernelGGL((grad_scan_kernel<T, V, LE, int32_t>), grid, dim3(256), 0, c.s, (const T*)c.g, c.stride, W,
                        (const int32_t*)c.ids, (int)c.n, c.rows, c.scale, (T*)c.out);
@@ -836,7 +871,8 @@ int launch_scan_le(const GradCall& c) {
 template <typename T, int V>
 int launch_scan(const GradCall& c) {
   const int64_t W = c.width / V;
-  if (W >= 48) return launch_scan_le<T, V, 64>(c);
+  // 64 lanes across the columns where that leaves workgroups enough, else 16 with four positions at a time
+  if (W >= 48 && (c.rows + 3) / 4 * ((W + 63) / 64) >= SCAN_BLOCKS / 2) return launch_scan_le<T, V, 64>(c);
   if (W >= 6) return launch_scan_le<T, V, 16>(c);
   if (W >= 2) return launch_scan_le<T, V, 4>(c);
   return launch_scan_le<T, V, 1>(c);
