@@ -436,17 +436,20 @@ __global__ __launch_bounds__(256) void grad_level_kernel(const S* __restrict__ s
                                                          const uint32_t* __restrict__ key, int64_t rows, int64_t n_blocks,
                                                          int bits, int span_bits, StartJob job,
                                                          float* __restrict__ sums) {
-  if (PERM && (int)blockIdx.x < job.blocks) return start_part(job);
+  if (PERM && (int)blockIdx.x < job.blocks) {
+    if (blockIdx.y == 0) start_part(job);
+    return;
+  }
   constexpr int Q = LE ? 64 / (LE ? LE : 1) : 1;
   const int per = LE ? 4 : 256 / tc, sub = LE ? threadIdx.x >> 6 : threadIdx.x / tc;
   const int t = LE ? threadIdx.x & 63 : threadIdx.x - sub * tc, step = LE ? LE : tc;
-  const int q = LE ? t / step : 0, col0 = LE ? t % step : t;
+  const int q = LE ? t / step : 0, col0 = blockIdx.y * step + (LE ? t % step : t), col_step = gridDim.y * step;
   if (sub >= per) return;
   const int64_t first = (int64_t)blockIdx.x - (PERM ? job.blocks : 0), step_blocks = (int64_t)gridDim.x - (PERM ? job.blocks : 0);
   for (int64_t b = first * per + sub; b < n_blocks; b += step_blocks * per) {
     const uint32_t k0 = key[b << span_bits];
     if (k0 != key[((b + 1) << span_bits) - 1] || k0 >= rows) continue;
-    for (int col = col0; col - col0 < W; col += step) {
+    for (int col = col0; col - (LE ? t % step : 0) < W; col += col_step) {     // by waves: all lanes as long as one has a column
       float acc[V] = {};
       if (col < W)
         grad_sum<S, V, PERM, Q, LE ? 8 : 4>(acc, src, stride, (int64_t)col * V, order, (int)(b << bits) + q,
@@ -457,6 +460,8 @@ __global__ __launch_bounds__(256) void grad_level_kernel(const S* __restrict__ s
   }
 }
 
+// blockIdx.y: columns beyond the first 256 vectors, where rows (or, above, blocks) are too few to fill the chip (2100
+// positions x 1999 columns into three rows: 114 -> 29 us).
 // A thread per vector; the next row's place in the order is on its way while this one's positions are added.  Vectors of
 // eight are added up in halves where a row has several positions: 64 registers instead of 86, eight waves instead of five
 // (65537 x 640 bf16 into 100003 rows 71 -> 62 us; where rows have six positions each, 300000 x 256 f16 into 50000, 53 -> 57).
@@ -465,7 +470,8 @@ __global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, 
                                                        const int32_t* __restrict__ order,
                                                        const int32_t* __restrict__ start, int64_t rows, GradLevels lv,
                                                        const float* __restrict__ sums, float scale, T* __restrict__ out) {
-  const int per_step = 256 / tc, sub = threadIdx.x / tc, col0 = threadIdx.x - sub * tc;
+  const int per_step = 256 / tc, sub = threadIdx.x / tc, col0 = blockIdx.y * tc + threadIdx.x - sub * tc;
+  const int col_step = gridDim.y * tc;
   int64_t r = (int64_t)blockIdx.x * per_step + sub;
   if (sub >= per_step || r >= rows) return;
   const int64_t width = (int64_t)W * V, step = (int64_t)gridDim.x * per_step;
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, 
     const int sn = start[next], en = start[next + 1];
     if (e - s <= 1) {                                    // most rows of a large table: one position or none
       const T* from = g + (e > s ? order[s] * stride : 0);
-      for (int col = col0; col < W; col += tc) {
+      for (int col = col0; col < W; col += col_step) {
         float acc[V] = {};
         if (e > s) {
           const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(from + (int64_t)col * V);
@@ -487,7 +493,7 @@ __global__ __launch_bounds__(256) void grad_row_kernel(const T* __restrict__ g, 
     } else {
       constexpr int H = V == 8 ? 4 : V, PARTS = V / H;
 #pragma unroll 1
-      for (int part = col0 * PARTS; part < W * PARTS; part += (part + 1) % PARTS ? 1 : (tc - 1) * PARTS + 1) {
+      for (int part = col0 * PARTS; part < W * PARTS; part += (part + 1) % PARTS ? 1 : (col_step - 1) * PARTS + 1) {
         const int64_t at = (int64_t)part * H;
         float acc[H] = {};
         grad_row_sum<T, H, 1, 3>(acc, g, stride, at, order, s, e, 0, width, lv, sums);
@@ -533,7 +539,7 @@ __global__ __launch_bounds__(256) void grad_row_wave_kernel(const T* __restrict_
 // rows: 5.5 us, one launch; ranking, the start of each row and the sums are three.  A list of more than SCAN_ALONE rounds
 // is shared by the workgroup's four waves, and where rows are few their columns go to workgroups of their own (each looks
 // through the ids again, 4 us): 2048 positions x 1999 columns into one row 45 us, x 2000 32; by one wave alone 11 ms and 2.1.
-constexpr int SCAN_MAX = 2048, SCAN_DEEP = 4, SCAN_ALONE = 4, SCAN_BLOCKS = 512;
+constexpr int SCAN_MAX = 2048, SCAN_DEEP = 4, SCAN_ALONE = 4;
 template <typename T, int V, int LE, typename I>
 __global__ __launch_bounds__(256) void grad_scan_kernel(const T* __restrict__ g, int64_t stride, int W,
                                                         const I* __restrict__ ids, int n, int64_t rows, float scale,
@@ -791,6 +797,14 @@ int64_t level_words(int64_t n, int64_t width, bool wave) {
 // whether looking through all ids for every row is the quickest way
 bool grad_by_scan(int64_t rows, int64_t n) { return n <= SCAN_MAX && rows * (n > 0 ? n : 1) <= (1 << 22); }
 
+// workgroups side by side for the columns of what `blocks` workgroups would take in `steps` steps: as long as the chip is
+// not full (two for each CU)
+constexpr int64_t FILL_BLOCKS = 512;
+unsigned column_blocks(int64_t blocks, int64_t steps) {
+  const int64_t wanted = FILL_BLOCKS / (blocks < 1 ? 1 : blocks);
+  return (unsigned)(wanted < 1 ? 1 : wanted < steps ? wanted : steps);
+}
+
 struct GradCall {
   const void* g;
   int64_t stride, n, width;
@@ -822,12 +836,13 @@ int launch_grad(const GradCall& c) {
     const int bits = l == 0 ? lv.chunk_bits : lv.fan_bits;
     const int64_t wanted = (lv.n[l] + per - 1) / per;
     const unsigned blocks = (unsigned)(wanted < (1 << 22) ? wanted : (1 << 22));
+    const unsigned columns = column_blocks(blocks, LE ? 1 : parts);
     span_bits += bits;
     if (l == 0)
-      hipLaunchKernelGGL((grad_level_kernel<T, V, LE, true>), dim3(blocks + job.blocks), dim3(256), 0, c.s, (const T*)c.g,
+      hipLaunchKernelGGL((grad_level_kernel<T, V, LE, true>), dim3(blocks + job.blocks, columns), dim3(256), 0, c.s, (const T*)c.g,
                          c.stride, W, tc, order, key, c.rows, lv.n[0], bits, span_bits, job, c.ws);
     else
-      hipLaunchKernelGGL((grad_level_kernel<float, V, LE, false>), dim3(blocks), dim3(256), 0, c.s, c.ws + lv.at[l - 1],
+      hipLaunchKernelGGL((grad_level_kernel<float, V, LE, false>), dim3(blocks, columns), dim3(256), 0, c.s, c.ws + lv.at[l - 1],
                          c.width, W, tc, order, key, c.rows, lv.n[l], bits, span_bits, none, c.ws + lv.at[l]);
   }
   if (LE) {
@@ -836,7 +851,8 @@ int launch_grad(const GradCall& c) {
                        dim3(256), 0, c.s, (const T*)c.g, c.stride, W, order, start, c.rows, lv, c.ws, c.scale, (T*)c.out);
   } else {
     const int64_t blocks = (c.rows + per - 1) / per;
-    hipLaunchKernelGGL((grad_row_kernel<T, V>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, c.s,
+    hipLaunchKernelGGL((grad_row_kernel<T, V>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), column_blocks(blocks, parts)),
+                       dim3(256), 0, c.s,
                        (const T*)c.g, c.stride, W, tc, order, start, c.rows, lv, c.ws, c.scale, (T*)c.out);
   }
   BVI_HIP_CHECK_LAUNCH();
@@ -856,9 +872,8 @@ int launch_grad_le(const GradCall& c) {
 template <typename T, int V, int LE>
 int launch_scan_le(const GradCall& c) {
   const int W = (int)(c.width / V);
-  // columns in workgroups of their own as long as the rows' do not fill the chip twice
-  const int64_t row_blocks = (c.rows + 3) / 4, steps = (W + (int64_t)LE - 1) / LE, wanted = SCAN_BLOCKS / row_blocks;
-  const dim3 grid((unsigned)row_blocks, (unsigned)(wanted < 1 ? 1 : wanted < steps ? wanted : steps));
+  const int64_t row_blocks = (c.rows + 3) / 4;
+  const dim3 grid((unsigned)row_blocks, column_blocks(row_blocks, (W + (int64_t)LE - 1) / LE));
   if (c.ids_type == BVI_IDS_I32)
     hipLaunchKernelGGL((grad_scan_kernel<T, V, LE, int32_t>), grid, dim3(256), 0, c.s, (const T*)c.g, c.stride, W,
                        (const int32_t*)c.ids, (int)c.n, c.rows, c.scale, (T*)c.out);
@@ -872,7 +887,7 @@ template <typename T, int V>
 int launch_scan(const GradCall& c) {
   const int64_t W = c.width / V;
   // 64 lanes across the columns where that leaves workgroups enough, else 16 with four positions at a time
-  if (W >= 48 && (c.rows + 3) / 4 * ((W + 63) / 64) >= SCAN_BLOCKS / 2) return launch_scan_le<T, V, 64>(c);
+  if (W >= 48 && (c.rows + 3) / 4 * ((W + 63) / 64) >= FILL_BLOCKS / 2) return launch_scan_le<T, V, 64>(c);
   if (W >= 6) return launch_scan_le<T, V, 16>(c);
   if (W >= 2) return launch_scan_le<T, V, 4>(c);
   return launch_scan_le<T, V, 1>(c);

@@ -353,14 +353,14 @@ def test_the_gradient_is_differentiable_in_what_it_adds_up(emb, gpu_device):
 
 
 WIDE = [(1, 1999, 2048), (1, 2000, 2048), (3, 1500, 1000), (2, 640, 2000), (1, 67, 2047), (5, 48, 1500), (9, 7, 2048), (2, 3, 2048),
-        (4, 1, 2048), (700, 1040, 2000), (1, 4097, 65)]
+        (4, 1, 2048), (700, 1040, 2000), (1, 4097, 65), (3, 1999, 2100), (1, 4100, 2300), (2, 2056, 5000), (40, 771, 2400)]
 
 
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
 @pytest.mark.parametrize('shape', WIDE, ids=str)
 def test_few_rows_of_many_positions(emb, gpu_device, shape, dtype):
     """Sizes that need no sort: rows that a workgroup shares and rows that a wave takes, in one call; columns in one
-    workgroup and in several; widths and strides of every vector."""
+    workgroup and in several; widths and strides of every vector.  And sizes just above, with columns in several too."""
     rows, width, n = shape
     rng = np.random.default_rng(n + width)
     gen = torch.Generator(device=gpu_device); gen.manual_seed(n)
@@ -375,9 +375,9 @@ def test_few_rows_of_many_positions(emb, gpu_device, shape, dtype):
 
 def test_wide_rows_of_many_positions_are_not_one_waves_work(emb, gpu_device):
     """2048 positions of 1999 columns in one row took 11 ms, index_add_ 0.08: within three times of it, by the fastest of
-    several runs each."""
+    several runs each.  Just above that number the sorted form's rows and blocks were one workgroup's work each."""
     import time
-    for rows, width, n in ((1, 1999, 2048), (1, 2000, 2048), (3, 1501, 1000)):
+    for rows, width, n in ((1, 1999, 2048), (1, 2000, 2048), (3, 1501, 1000), (3, 1999, 2100)):
         gen = torch.Generator(device=gpu_device); gen.manual_seed(n)
         g = torch.randn(n, width, generator=gen, device=gpu_device)
         ids = torch.randint(0, rows, (n,), generator=gen, device=gpu_device)
