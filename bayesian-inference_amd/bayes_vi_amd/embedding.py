@@ -37,7 +37,7 @@ def _rows_view(t, what):
 
 def _differentiated(t):
     """Whether autograd follows t: backwards, or forwards by a tangent (which `requires_grad` says nothing about)."""
-    return (torch.is_grad_enabled() and t.requires_grad
+    return (t.requires_grad and torch.is_grad_enabled()
             or _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None)
 
 
@@ -80,11 +80,10 @@ def lookup_grad(grad_out, ids, num_rows, scale=1.0, plan=None):
         plan.check(ids.numel(), num_rows, grad_out.device)
     if _differentiated(grad_out):
         return _LookupGrad.apply(grad_out, ids, num_rows, float(scale), plan)
-    return _gradient(grad_out, ids, num_rows, float(scale), plan)
+    return _gradient(grad_out, ids, num_rows, float(scale), plan, flat)
 
 
-def _gradient(grad_out, ids, num_rows, scale, plan):
-    flat = grad_out.dim() == ids.dim()
+def _gradient(grad_out, ids, num_rows, scale, plan, flat):
     n, width = ids.numel(), 1 if flat else grad_out.shape[-1]
     g, stride = _rows_view(grad_out.reshape(n, width), 'grad_out')
     ids = ids.contiguous()
@@ -127,7 +126,7 @@ class _LookupGrad(torch.autograd.Function):
         ctx.rows, ctx.scale, ctx.plan = num_rows, scale, plan
         ctx.save_for_backward(ids)
         ctx.save_for_forward(ids)
-        return _gradient(grad_out, ids, num_rows, scale, plan)
+        return _gradient(grad_out, ids, num_rows, scale, plan, grad_out.dim() == ids.dim())
 
     @staticmethod
     def backward(ctx, grad_table):
