@@ -723,9 +723,12 @@ void launch_passes(const GrCall& c, bool grad) {
   }
 }
 // whether the tables are copied to [group, chain] first: a row's own entry comes once per group, those of other lookups
-// by gathers of a line per chain (300001 rows, 20000 and 60 groups, 4 chains: the passes take 25 us beside a copy of 5 and
-// 23 without it)
-bool transposes(int lookups, int C) { return lookups > 1 && C > 4; }
+// by gathers of a line per chain.  us a call without / with the copy, 300001 rows:
+//   20000 and 60 groups, D = 3     4 chains 36.0 / 37.5,  8 chains 76.9 / 78.5,  16 chains 87.6 / 84.7,  64 chains 187 / 125
+//   2000 and 2000 groups           26.2 / 29.4,           41.6 / 45.0,           53.4 / 46.8,            183 / 96
+//   200000 and 50000, D = 2        47.0 / 53.2,           110 / 115,             166 / 122,              988 / 293
+// (2000 rows, where nothing but launches counts, 16 chains 19 / 22, 64 chains 23 / 30)
+bool transposes(int lookups, int C) { return lookups > 1 && C > 8; }
 
 }  // namespace
 
