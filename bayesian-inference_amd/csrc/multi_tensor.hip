@@ -192,7 +192,19 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restri
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// every workgroup adds up the same partial sums (at most a few KB from L2) instead of waiting for a launch that does.
+// The partial sums of a list of several batches, added up once (in the order in which clip_kernel adds those of one): every
+// workgroup of every batch's clipping would read all of them (1600 tensors of 40000 elements: 160 KB each; the 20 launches 334 -> 200 us).
+__global__ __launch_bounds__(256) void norm_join_kernel(const double* __restrict__ part, int n_part,
+                                                        double* __restrict__ total) {
+  __shared__ double red[4];
+  double s = 0.0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n_part; i += 256) s += part[i];
+  s = mt_block_sum(s, red);
+  if (threadIdx.x == 0) *total = s;
+}
+
+// every workgroup adds up the same partial sums (at most 8 KB from L2) instead of waiting for a launch that does.
 // One read and one write: the same 58M values 68 us = 6.4 TB/s.
 template <bool PAST_CACHE>
 __global__ __launch_bounds__(256) void clip_kernel(ClipArgs a, const double* __restrict__ part, int n_part,
@@ -357,8 +369,8 @@ __device__ __forceinline__ void adam_update(float* __restrict__ x, float* __rest
   }
 }
 
-// Four arrays read, three or (where a factor is not one) four written: 29M variables, 937 MB, 144 us = 6.5 TB/s.  Only
-// bytes count; the norm pass before it is the fifth read, since every variable's norm is needed before its first step.
+// Four arrays read, three or (where a factor is not one) four written: 29M elements 146 us for 820 MB = 5.6 TB/s, or 160 us
+// for 937 MB = 5.9 TB/s.  Only bytes count; the norm pass before it is the fifth read, since every variable's norm is needed before its first step.
 __global__ __launch_bounds__(256) void adam_update_kernel(AdamArgs a, AdamHyper h, const float* __restrict__ factor,
                                                           const double* __restrict__ state) {
   const float joint = (float)state[1], lr_t = (float)state[2];
@@ -495,7 +507,7 @@ extern "C" {
 
 int bvi_global_norm_ws_bytes(int n_tensors, size_t* ws_bytes) {
   if (!ws_bytes || n_tensors < 1) return BVI_ERR_ARG;
-  *ws_bytes = (size_t)batches_of(n_tensors) * MT_BLOCKS * sizeof(double);
+  *ws_bytes = ((size_t)batches_of(n_tensors) * MT_BLOCKS + 1) * sizeof(double);
   return BVI_OK;
 }
 
@@ -550,6 +562,13 @@ int bvi_clip_by_global_norm(int n_tensors, const void* const* tensors, void* con
     const int st = launch_norm(n_tensors, tensors, sizes, dtypes, (double*)ws, &n_part, s);
     if (st) return st;
   }
+  const double* part = (const double*)ws;
+  if (n_part > MT_BLOCKS) {
+    double* total = (double*)((char*)ws + need) - 1;
+    hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, s, part, n_part, total);
+    part = total;
+    n_part = 1;
+  }
   // results beyond the 32 MB of L2 go past the caches: 58M values 70 -> 66 us here, and 42 -> 33 us in the next norm pass
   // over the same gradients
   int64_t bytes = 0;
@@ -562,10 +581,10 @@ int bvi_clip_by_global_norm(int n_tensors, const void* const* tensors, void* con
     const dim3 grid(blocks_for(a.in.first[a.in.count], 2 * MT_BLOCKS));
     float* norm_out = t0 == 0 ? norm : nullptr;
     if (past_cache)
-      hipLaunchKernelGGL(clip_kernel<true>, grid, dim3(256), 0, s, a, (const double*)ws, n_part, use_norm,
+      hipLaunchKernelGGL(clip_kernel<true>, grid, dim3(256), 0, s, a, part, n_part, use_norm,
                          (double)clip_norm, norm_out);
     else
-      hipLaunchKernelGGL(clip_kernel<false>, grid, dim3(256), 0, s, a, (const double*)ws, n_part, use_norm,
+      hipLaunchKernelGGL(clip_kernel<false>, grid, dim3(256), 0, s, a, part, n_part, use_norm,
                          (double)clip_norm, norm_out);
   }
   BVI_HIP_CHECK_LAUNCH();

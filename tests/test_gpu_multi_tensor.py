@@ -275,3 +275,28 @@ def test_the_norm_to_use_may_not_be_written(la, gpu_device):
     assert float(norm) == 3.0 and bool((out[0] == 1).all())
     la.clip_by_global_norm([t[:7]], 1.0, use_norm=t[7], inplace=True)    # beside the tensor: fine
     assert bool((t[:7] == 1).all()) and bool((t[7:] == 3).all())
+
+
+def test_lists_of_many_launches(la, gpu_device):
+    """Tensors beyond what one launch's arguments hold, large enough for several workgroups each: the norm and the clipped
+    values, in place and apart, and again the same bits from a graph."""
+    for count, n in ((81, 60_000), (400, 5_000)):
+        ts = tensors([(n + k % 3,) for k in range(count)], [torch.float32, torch.bfloat16] * count, 0.5, count, gpu_device)
+        s = norm64(ts)
+        out, norm = la.clip_by_global_norm(ts, 0.25 * s)
+        assert abs(float(norm) - s) <= 2 * U * s and abs(float(la.global_norm(ts)) - s) <= 2 * U * s
+        for o, t in zip(out, ts):
+            f = torch.finfo(t.dtype)
+            ref = t.double() * 0.25
+            assert bool(((o.double() - ref).abs() <= (f.eps / 2 + 4 * U) * ref.abs() + f.smallest_normal * f.eps).all())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again, norm2 = la.clip_by_global_norm(ts, 0.25 * s)
+        for _ in range(3):
+            graph.replay()
+            eager, _ = la.clip_by_global_norm(ts, 0.25 * s)
+            assert torch.equal(norm2, norm) and all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(again, out, eager))
+        own = [t.clone() for t in ts]
+        la.clip_by_global_norm(own, 0.25 * s, inplace=True)
+        assert all(torch.equal(a, b) for a, b in zip(own, out))
