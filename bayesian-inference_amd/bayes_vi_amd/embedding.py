@@ -4,7 +4,8 @@ bvi_lookup_grad).  `symbolic.gather` is the spelling for likelihood callables.
 
 Tables are [rows, width] (or [rows]) in float32, bfloat16 or float16 with any row stride; ids int32 or int64 of any shape.
 An id outside [0, rows) is padding: it reads zeros and takes no part in the gradient.  Products and sums are in float32,
-rounded once to the table's type.  Everything runs on the current stream of the table's device; nothing synchronises, and
+rounded once to the table's type.  Derivatives go backwards and forwards (torch.autograd, forward_ad); torch.func
+transforms raise.  Everything runs on the current stream of the table's device; nothing synchronises, and
 every call can be recorded into a graph.
 """
 from __future__ import annotations

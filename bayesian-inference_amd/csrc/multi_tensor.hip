@@ -192,8 +192,9 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restri
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// The partial sums of a list of several batches, added up once (in the order in which clip_kernel adds those of one): every
-// workgroup of every batch's clipping would read all of them (1600 tensors of 40000 elements: 160 KB each; the 20 launches 334 -> 200 us).
+// The partial sums of a list of several launches, added up once (in the order in which clip_kernel adds those of one): every
+// workgroup of every launch would read all of them (1600 tensors of 40000 elements: 160 KB each, the 20 clipping launches
+// 334 us, with one sum beforehand 200 + 6).
 __global__ __launch_bounds__(256) void norm_join_kernel(const double* __restrict__ part, int n_part,
                                                         double* __restrict__ total) {
   __shared__ double red[4];
@@ -208,7 +209,8 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const double* __restrict
 // One read and one write: the same 58M values 68 us = 6.4 TB/s.
 template <bool PAST_CACHE>
 __global__ __launch_bounds__(256) void clip_kernel(ClipArgs a, const double* __restrict__ part, int n_part,
-                                                   const float* __restrict__ use_norm, double clip, float* __restrict__ norm_out) {
+                                                   const float* __restrict__ use_norm, double clip,
+                                                   float* __restrict__ norm_out) {
   __shared__ double red[4];
   double norm;
   if (use_norm) {
@@ -370,7 +372,8 @@ __device__ __forceinline__ void adam_update(float* __restrict__ x, float* __rest
 }
 
 // Four arrays read, three or (where a factor is not one) four written: 29M elements 146 us for 820 MB = 5.6 TB/s, or 160 us
-// for 937 MB = 5.9 TB/s.  Only bytes count; the norm pass before it is the fifth read, since every variable's norm is needed before its first step.
+// for 937 MB = 5.9 TB/s.  Only bytes count; the norm pass before it is the fifth read, since every variable's norm is needed
+// before its first step.
 __global__ __launch_bounds__(256) void adam_update_kernel(AdamArgs a, AdamHyper h, const float* __restrict__ factor,
                                                           const double* __restrict__ state) {
   const float joint = (float)state[1], lr_t = (float)state[2];
